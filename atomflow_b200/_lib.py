@@ -53,6 +53,27 @@ class ChainOp(ctypes.Structure):
                 ("aux", ctypes.c_void_p)]
 
 
+class KvFormat(enum.IntEnum):
+    F16 = 0
+    FP8_E4M3 = 1
+    INT8 = 2
+
+
+class PagedKv(ctypes.Structure):
+    """af_paged_kv (include/atomflow_b200.h)."""
+    _fields_ = [("format", ctypes.c_int), ("n_pages", ctypes.c_int), ("page_size", ctypes.c_int),
+                ("n_kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("k", ctypes.c_void_p),
+                ("v", ctypes.c_void_p), ("page_stride", ctypes.c_int64), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("scale_stride", ctypes.c_int64)]
+
+
+class PagedBatch(ctypes.Structure):
+    """af_paged_batch (include/atomflow_b200.h)."""
+    _fields_ = [("n_seqs", ctypes.c_int), ("n_tokens", ctypes.c_int), ("max_pages", ctypes.c_int),
+                ("cu_rows", ctypes.c_void_p), ("kv_len", ctypes.c_void_p), ("block_table", ctypes.c_void_p),
+                ("table_stride", ctypes.c_int64)]
+
+
 class OpKind(enum.IntEnum):
     GEMV = 0
     GEMV_RESIDUAL = 1
@@ -63,6 +84,7 @@ class OpKind(enum.IntEnum):
 # Every symbol include/atomflow_b200.h and include/atomflow_view_ops.h declare,
 # with its ctypes signature (restype, argtypes).
 _vp, _sz, _i, _fp = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_void_p
+_i64 = ctypes.c_int64
 C_SYMBOLS = {
     "af_status_string": (ctypes.c_char_p, [_i]),
     "af_last_cuda_error": (ctypes.c_char_p, []),
@@ -104,6 +126,9 @@ C_SYMBOLS = {
     "af_chain_workspace_bytes": (_sz, [_i]),
     "af_gemv_chain": (_i, [ctypes.c_void_p, _i, _vp, _sz, _vp]),
     "af_gemv_chain_fast": (_i, [ctypes.c_void_p, _i, _vp, _sz, _vp]),
+    "af_paged_kv_write": (_i, [_vp, _vp, _vp, _i64, _i, _vp, _vp, _i, _vp, _vp]),
+    "af_paged_kv_read": (_i, [_vp, _vp, _vp, _vp, _vp]),
+    "af_paged_attention": (_i, [_vp, _vp, _vp, _i64, _i, ctypes.c_float, _i, _i, _vp, _vp]),
     "af_engine_create": (_i, [ctypes.c_char_p, _i, _i, _i, ctypes.POINTER(ctypes.c_void_p)]),
     "af_engine_create_tp": (_i, [ctypes.c_char_p, _i, _i, _vp, ctypes.POINTER(ctypes.c_void_p)]),
     "af_engine_destroy": (_i, [_vp]),

@@ -26,6 +26,7 @@ unsigned gemv_faults(bool clear, cudaError_t* err);
 unsigned decode_faults(bool clear, cudaError_t* err);
 unsigned chain_faults(bool clear, cudaError_t* err);
 unsigned tc_faults(bool clear, cudaError_t* err);
+unsigned paged_faults(bool clear, cudaError_t* err);
 // 8+ token FP8 projections on the tcgen05 tensor cores (af_gemv_tc.cu)
 bool tc_ok(int M, int K, bool row_scale, const void* x, const void* w, const void* s, const void* y);
 af_status tc_launch(const void* x, const void* w, const void* s, bool row_scale, void* y, int M, int N, int K,

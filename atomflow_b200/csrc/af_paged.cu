@@ -1,0 +1,435 @@
+// af_paged.cu -- a KV cache in pages for a batch of sequences: rotate, quantise
+// and store new tokens (af_paged_kv_write), read positions back
+// (af_paged_kv_read), attend over the pages (af_paged_attention).
+//
+// The batched, paged counterparts of af_rope_kv_write and af_decode_attention:
+// one page is a stretch of the same token-major rows [NKV * HD] that the
+// one-sequence cache has, so a contiguous cache is a pool whose table counts up.
+#include "af_paged.cuh"
+
+using namespace af;
+
+// Fault bits (AF_FAULT_*) of this device's paged kernels, read by af_device_faults.
+__device__ unsigned int g_paged_faults;
+
+namespace {
+
+// ---------------------------------------------------------------- write
+// One CTA per token.  HD / 8 lanes hold one head's vector, lane l the pairs
+// (4l + i, 4l + i + HD/2): RoPE's partner is in the same thread, and each load
+// and store of the lanes is one contiguous run.  Bound by DRAM: the qkv rows in,
+// q and the codes out.  The loads of a thread's vectors are issued before the
+// token's sequence is searched, so the search hides behind them.
+constexpr int kWriteThreads = 256;
+constexpr int kWriteBatch = 3;   // vectors of one thread in flight: 48 per CTA pass at HD 128
+
+struct WriteArgs {
+    const __half* qkv;
+    long long stride;        // elements from one token's row to the next
+    const float *cos, *sin;  // [max_seq][HD / 2], or NULL: no rotation
+    __half* q_out;
+    int NH, max_seq;
+};
+
+// The framework's rotation (rope.cu of the reference, its fast-math contraction):
+// the same two roundings as af_rope_kv_write.
+__device__ __forceinline__ void rope_pair(float x, float y, float c, float s, float& o0, float& o1) {
+    o0 = fmaf(x, c, -__fmul_rn(y, s));
+    o1 = fmaf(x, s, __fmul_rn(y, c));
+}
+
+template <int FMT, int HD>
+__global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const Paged p, const WriteArgs a,
+                                                                    unsigned* fault) {
+    constexpr int L = HD / 8, GROUPS = kWriteThreads / L, HALF = HD / 2;
+    const int t = blockIdx.x, grp = threadIdx.x / L, l = threadIdx.x % L;
+    const bool rotate = a.cos != nullptr;
+    const int first = rotate ? 0 : a.NH, nvec = a.NH + 2 * p.NKV;   // without rotation q stays where it is
+    const __half* row = a.qkv + (long long)t * a.stride;
+    uint2 lo[kWriteBatch], hi[kWriteBatch];
+    auto load = [&](int v0) {
+#pragma unroll
+        for (int i = 0; i < kWriteBatch; ++i) {
+            const int v = v0 + i * GROUPS;
+            if (v < nvec) {
+                lo[i] = __ldg(reinterpret_cast<const uint2*>(row + (long long)v * HD + 4 * l));
+                hi[i] = __ldg(reinterpret_cast<const uint2*>(row + (long long)v * HD + HALF + 4 * l));
+            }
+        }
+    };
+    load(first + grp);
+    const int b = paged_find(p, t);
+    const PagedSeq s = paged_seq(p, b, fault);
+    const int pos = s.kv - s.q + (t - s.row0);
+    if (t < s.row0 || t >= s.row0 + s.q || pos < 0) return;   // no sequence's row, or before position 0
+    if (rotate && pos >= a.max_seq) {
+        if (threadIdx.x == 0) atomicOr(fault, (unsigned)AF_FAULT_POSITION);
+        return;
+    }
+    const int page = paged_page(p, b, pos, fault);
+    if (page < 0) return;
+    float4 c = make_float4(1.f, 1.f, 1.f, 1.f), sn = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (rotate) {
+        c = __ldg(reinterpret_cast<const float4*>(a.cos + (long long)pos * HALF) + l);
+        sn = __ldg(reinterpret_cast<const float4*>(a.sin + (long long)pos * HALF) + l);
+    }
+    const float ca[4] = {c.x, c.y, c.z, c.w}, sa[4] = {sn.x, sn.y, sn.z, sn.w};
+    for (int v0 = first + grp; v0 < nvec; v0 += kWriteBatch * GROUPS) {
+        if (v0 != first + grp) load(v0);
+#pragma unroll
+        for (int i = 0; i < kWriteBatch; ++i) {
+            const int v = v0 + i * GROUPS;
+            if (v - grp >= nvec) break;   // uniform over the warp: the shuffles below take every lane
+            const bool on = v < nvec;
+            if (!on) lo[i] = hi[i] = make_uint2(0u, 0u);
+            const bool is_v = v >= a.NH + p.NKV;
+            if (rotate && !is_v) {
+                __half2* pl = reinterpret_cast<__half2*>(&lo[i]);
+                __half2* ph = reinterpret_cast<__half2*>(&hi[i]);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float2 x = __half22float2(pl[j]), y = __half22float2(ph[j]);
+                    float2 r0, r1;
+                    rope_pair(x.x, y.x, ca[2 * j], sa[2 * j], r0.x, r1.x);
+                    rope_pair(x.y, y.y, ca[2 * j + 1], sa[2 * j + 1], r0.y, r1.y);
+                    pl[j] = __float22half2_rn(r0);
+                    ph[j] = __float22half2_rn(r1);
+                }
+            }
+            const int h = v - a.NH - (is_v ? p.NKV : 0);   // kv head; negative for q
+            const long long slot = (long long)paged_slot(p, pos) * p.NKV + h;
+            uint8_t* dst = (is_v ? p.v : p.k) + (long long)page * p.page_bytes +
+                           slot * (HD * KvFormat<FMT>::kBytes);
+            if constexpr (FMT == AF_KV_F16) {
+                if (on) {
+                    __half* out = v < a.NH ? a.q_out + ((long long)t * a.NH + v) * HD : reinterpret_cast<__half*>(dst);
+                    *reinterpret_cast<uint2*>(out + 4 * l) = lo[i];
+                    *reinterpret_cast<uint2*>(out + HALF + 4 * l) = hi[i];
+                }
+            } else {
+                float x[4], y[4];
+                const __half2* pl = reinterpret_cast<const __half2*>(&lo[i]);
+                const __half2* ph = reinterpret_cast<const __half2*>(&hi[i]);
+                float amax = 0.f;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float2 u = __half22float2(pl[j]), w = __half22float2(ph[j]);
+                    x[2 * j] = u.x;
+                    x[2 * j + 1] = u.y;
+                    y[2 * j] = w.x;
+                    y[2 * j + 1] = w.y;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) amax = fmaxf(amax, fmaxf(fabsf(x[j]), fabsf(y[j])));
+#pragma unroll
+                for (int o = L / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                if (on && v < a.NH) {
+                    __half* out = a.q_out + ((long long)t * a.NH + v) * HD;
+                    *reinterpret_cast<uint2*>(out + 4 * l) = lo[i];
+                    *reinterpret_cast<uint2*>(out + HALF + 4 * l) = hi[i];
+                } else if (on) {
+                    const __half sc = kv_scale<FMT>(amax);
+                    const float f = __half2float(sc);
+                    *reinterpret_cast<uint32_t*>(dst + 4 * l) = kv_pack4<FMT>(x, f);
+                    *reinterpret_cast<uint32_t*>(dst + HALF + 4 * l) = kv_pack4<FMT>(y, f);
+                    if (l == 0) (is_v ? p.vs : p.ks)[(long long)page * p.scale_stride + slot] = sc;
+                }
+            }
+        }
+    }
+}
+
+// ----------------------------------------------------------------- read
+// Rows of positions -> contiguous FP16.  A CTA takes kReadRows rows; each
+// thread moves 16-byte pieces (one piece of an 8-bit cache makes two of FP16).
+// Bound by DRAM: codes in, FP16 out.
+constexpr int kReadThreads = 256;
+constexpr int kReadRows = 8;
+constexpr int kReadBatch = 4;
+
+template <int FMT, int HD>
+__global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const Paged p, __half* __restrict__ k_out,
+                                                                  __half* __restrict__ v_out, unsigned* fault) {
+    __shared__ long long s_at[kReadRows];    // page * 2^32 + slot of each row; -1: zeros; -2: not ours
+    const int t0 = blockIdx.x * kReadRows;
+    if (threadIdx.x < kReadRows) {
+        const int t = t0 + threadIdx.x;
+        long long at = -2;
+        if (t < p.n_tokens) {
+            const int b = paged_find(p, t);
+            const PagedSeq s = paged_seq(p, b, fault);
+            if (t >= s.row0 && t < s.row0 + s.q) {
+                const int pos = s.kv - s.q + (t - s.row0);
+                const int page = pos < 0 ? -1 : paged_page(p, b, pos, fault);
+                at = page < 0 ? -1 : ((long long)page << 32) | paged_slot(p, pos);
+            }
+        }
+        s_at[threadIdx.x] = at;
+    }
+    __syncthreads();
+    constexpr int PER = HD * KvFormat<FMT>::kBytes / 16;   // pieces of one vector
+    const int pieces = p.NKV * PER;                        // of one row of K (or V)
+    const int total = kReadRows * 2 * pieces;
+    for (int i0 = threadIdx.x; i0 < total; i0 += kReadBatch * kReadThreads) {
+        uint4 x[kReadBatch];
+        __half sc[kReadBatch];
+#pragma unroll
+        for (int j = 0; j < kReadBatch; ++j) {
+            const int i = i0 + j * kReadThreads;
+            x[j] = make_uint4(0u, 0u, 0u, 0u);
+            sc[j] = __float2half_rn(0.f);
+            if (i >= total) continue;
+            const int r = i / (2 * pieces), w = i % (2 * pieces), piece = w % pieces;
+            const bool is_v = w >= pieces;
+            const long long at = s_at[r];
+            if (at < 0) continue;
+            const long long page = at >> 32, slot = at & 0xffffffff;
+            x[j] = ldg_stream((is_v ? p.v : p.k) + page * p.page_bytes + (slot * pieces + piece) * 16);
+            if constexpr (FMT != AF_KV_F16)
+                sc[j] = __ldg((is_v ? p.vs : p.ks) + page * p.scale_stride + slot * p.NKV + piece / PER);
+        }
+#pragma unroll
+        for (int j = 0; j < kReadBatch; ++j) {
+            const int i = i0 + j * kReadThreads;
+            if (i >= total) continue;
+            const int r = i / (2 * pieces), w = i % (2 * pieces), piece = w % pieces;
+            if (s_at[r] == -2) continue;
+            __half* out = (w >= pieces ? v_out : k_out) + (long long)(t0 + r) * p.NKV * HD +
+                          (long long)piece * (16 / KvFormat<FMT>::kBytes);
+            if constexpr (FMT == AF_KV_F16) {
+                *reinterpret_cast<uint4*>(out) = x[j];
+            } else {
+                const __half2 s2 = __half2half2(sc[j]);
+                uint32_t o[8];
+                const uint32_t in[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    kv_unpack4<FMT>(in[q], o[2 * q], o[2 * q + 1]);
+                    o[2 * q] = mul_half2(o[2 * q], s2);
+                    o[2 * q + 1] = mul_half2(o[2 * q + 1], s2);
+                }
+                reinterpret_cast<uint4*>(out)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+                reinterpret_cast<uint4*>(out)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------ attention
+// One warp per (token, query head): online softmax over the positions it sees,
+// HD / 32 dims per lane.
+constexpr int kAttnWarps = 4;
+
+template <int FMT, int HD>
+__global__ void __launch_bounds__(kAttnWarps * 32) paged_attention_kernel(const Paged p, const __half* __restrict__ q,
+                                                                          long long q_stride, __half* __restrict__ out,
+                                                                          int NH, float scale, unsigned* fault) {
+    constexpr int E = HD / 32;
+    const int t = blockIdx.x, lane = threadIdx.x & 31, h = blockIdx.y * kAttnWarps + (threadIdx.x >> 5);
+    if (h >= NH) return;
+    const int kvh = h / (NH / p.NKV);
+    const int b = paged_find(p, t);
+    const PagedSeq s = paged_seq(p, b, fault);
+    if (t < s.row0 || t >= s.row0 + s.q) return;
+    const int end = s.kv - s.q + (t - s.row0) + 1;
+    float qv[E], o[E], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        qv[e] = __half2float(q[(long long)t * q_stride + h * HD + lane * E + e]) * scale;
+        o[e] = 0.f;
+    }
+    for (int j = 0; j < end; ++j) {
+        const int page = paged_page(p, b, j, fault);
+        const long long slot = (long long)paged_slot(p, j) * p.NKV + kvh;
+        float k[E], v[E];
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            float* x = w ? v : k;
+            const uint8_t* src = (w ? p.v : p.k) + (long long)page * p.page_bytes +
+                                 (slot * HD + lane * E) * KvFormat<FMT>::kBytes;
+            float sc = 1.f;
+            if constexpr (FMT != AF_KV_F16)
+                if (page >= 0) sc = __half2float((w ? p.vs : p.ks)[(long long)page * p.scale_stride + slot]);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                x[e] = 0.f;
+                if (page < 0) continue;
+                if constexpr (FMT == AF_KV_F16) x[e] = __half2float(reinterpret_cast<const __half*>(src)[e]);
+                else if constexpr (FMT == AF_KV_INT8) x[e] = (float)reinterpret_cast<const int8_t*>(src)[e] * sc;
+                else x[e] = (float)reinterpret_cast<const __nv_fp8_e4m3*>(src)[e] * sc;
+            }
+        }
+        float d = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) d = fmaf(qv[e], k[e], d);
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
+        const float mn = fmaxf(m, d), corr = __expf(m - mn), w = __expf(d - mn);
+        l = fmaf(l, corr, w);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = fmaf(w, v[e], o[e] * corr);
+        m = mn;
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) out[((long long)t * NH + h) * HD + lane * E + e] = __float2half_rn(o[e] * inv);
+}
+
+}  // namespace
+
+namespace af {
+
+unsigned* paged_fault_word(cudaError_t* err) {
+    static unsigned* word[kMaxDevices];   // benign race: every writer stores the same address
+    int dev = 0;
+    *err = cudaGetDevice(&dev);
+    if (*err != cudaSuccess || dev < 0 || dev >= kMaxDevices) return nullptr;
+    if (word[dev] == nullptr) {
+        void* ptr = nullptr;
+        *err = cudaGetSymbolAddress(&ptr, g_paged_faults);
+        if (*err != cudaSuccess) return nullptr;
+        word[dev] = static_cast<unsigned*>(ptr);
+    }
+    return word[dev];
+}
+
+unsigned paged_faults(bool clear, cudaError_t* err) {
+    unsigned v = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&v, g_paged_faults, sizeof(v));
+    if (e == cudaSuccess && clear && v != 0) {
+        const unsigned z = 0;
+        e = cudaMemcpyToSymbol(g_paged_faults, &z, sizeof(z));
+    }
+    *err = e;
+    return v;
+}
+
+af_status paged_args(const af_paged_kv* kv, const af_paged_batch* batch, Paged* out) {
+    if (kv == nullptr || batch == nullptr) return AF_ERR_INVALID;
+    if (kv->format != AF_KV_F16 && kv->format != AF_KV_FP8_E4M3 && kv->format != AF_KV_INT8) return AF_ERR_INVALID;
+    if (kv->head_dim != 64 && kv->head_dim != 128) return AF_ERR_UNSUPPORTED;
+    if (kv->n_pages < 0 || kv->n_kv_heads < 1 || kv->n_kv_heads > 1024) return AF_ERR_INVALID;
+    const int ps = kv->page_size;
+    if (ps < kPagedMinPage || ps > kPagedMaxPage || (ps & (ps - 1)) != 0) return AF_ERR_UNSUPPORTED;
+    if (batch->n_seqs < 0 || batch->n_tokens < 0 || batch->max_pages < 0) return AF_ERR_INVALID;
+    const bool quant = kv->format != AF_KV_F16;
+    if (!quant && (kv->k_scale != nullptr || kv->v_scale != nullptr)) return AF_ERR_INVALID;
+    const long long esz = quant ? 1 : 2;
+    const long long row = (long long)kv->n_kv_heads * kv->head_dim;
+    if (kv->page_stride < ps * row || (kv->page_stride * esz) % 16 != 0) return AF_ERR_INVALID;
+    if (quant && kv->scale_stride < (long long)ps * kv->n_kv_heads) return AF_ERR_INVALID;
+    if (batch->table_stride < batch->max_pages) return AF_ERR_INVALID;
+    if (batch->n_seqs > 0 && batch->n_tokens > 0) {
+        if (kv->k == nullptr || kv->v == nullptr || !aligned(kv->k, 16) || !aligned(kv->v, 16)) return AF_ERR_INVALID;
+        if (quant && (kv->k_scale == nullptr || kv->v_scale == nullptr || !aligned(kv->k_scale, 2) ||
+                      !aligned(kv->v_scale, 2)))
+            return AF_ERR_INVALID;
+        if (batch->cu_rows == nullptr || batch->kv_len == nullptr || !aligned(batch->cu_rows, 4) ||
+            !aligned(batch->kv_len, 4))
+            return AF_ERR_INVALID;
+        if (batch->max_pages > 0 && (batch->block_table == nullptr || !aligned(batch->block_table, 4)))
+            return AF_ERR_INVALID;
+    }
+    int shift = 0;
+    while ((1 << shift) < ps) ++shift;
+    out->k = static_cast<uint8_t*>(kv->k);
+    out->v = static_cast<uint8_t*>(kv->v);
+    out->ks = static_cast<__half*>(kv->k_scale);
+    out->vs = static_cast<__half*>(kv->v_scale);
+    out->page_bytes = kv->page_stride * esz;
+    out->scale_stride = kv->scale_stride;
+    out->cu = batch->cu_rows;
+    out->len = batch->kv_len;
+    out->table = batch->block_table;
+    out->table_stride = batch->table_stride;
+    out->n_pages = kv->n_pages;
+    out->page_shift = shift;
+    out->NKV = kv->n_kv_heads;
+    out->n_seqs = batch->n_seqs;
+    out->n_tokens = batch->n_tokens;
+    out->max_pages = batch->max_pages;
+    return AF_OK;
+}
+
+// Calls f<FMT, HD>() for the cache's format and head size (checked by paged_args).
+template <class F>
+static void paged_dispatch(const af_paged_kv* kv, F&& f) {
+    auto hd = [&](auto fmt) {
+        if (kv->head_dim == 128) f(fmt, std::integral_constant<int, 128>());
+        else f(fmt, std::integral_constant<int, 64>());
+    };
+    if (kv->format == AF_KV_F16) hd(std::integral_constant<int, AF_KV_F16>());
+    else if (kv->format == AF_KV_FP8_E4M3) hd(std::integral_constant<int, AF_KV_FP8_E4M3>());
+    else hd(std::integral_constant<int, AF_KV_INT8>());
+}
+
+}  // namespace af
+
+extern "C" af_status af_paged_kv_write(const af_paged_kv* kv, const af_paged_batch* batch, const void* qkv,
+                                       int64_t qkv_stride, int n_heads, const float* cos_tab, const float* sin_tab,
+                                       int max_seq, void* q_out, void* stream) {
+    Paged p;
+    const af_status st = paged_args(kv, batch, &p);
+    if (st != AF_OK) return st;
+    if (n_heads < 0 || n_heads > 65535 || (cos_tab == nullptr) != (sin_tab == nullptr)) return AF_ERR_INVALID;
+    if (qkv_stride < (int64_t)(n_heads + 2 * p.NKV) * kv->head_dim || qkv_stride % 8 != 0) return AF_ERR_INVALID;
+    if (cos_tab != nullptr && (max_seq < 1 || !aligned(cos_tab, 16) || !aligned(sin_tab, 16))) return AF_ERR_INVALID;
+    if (p.n_seqs == 0 || p.n_tokens == 0) return AF_OK;
+    if (qkv == nullptr || !aligned(qkv, 16)) return AF_ERR_INVALID;
+    if (cos_tab != nullptr && n_heads > 0 && (q_out == nullptr || !aligned(q_out, 16))) return AF_ERR_INVALID;
+    cudaError_t e;
+    unsigned* fault = paged_fault_word(&e);
+    if (fault == nullptr) return cuda_fail(e, "af_paged_kv_write");
+    const WriteArgs a{static_cast<const __half*>(qkv), qkv_stride, cos_tab, sin_tab, static_cast<__half*>(q_out),
+                      n_heads, max_seq};
+    paged_dispatch(kv, [&](auto fmt, auto hd) {
+        paged_write_kernel<decltype(fmt)::value, decltype(hd)::value>
+            <<<p.n_tokens, kWriteThreads, 0, static_cast<cudaStream_t>(stream)>>>(p, a, fault);
+    });
+    e = cudaGetLastError();
+    return e == cudaSuccess ? AF_OK : cuda_fail(e, "paged_write_kernel");
+}
+
+extern "C" af_status af_paged_kv_read(const af_paged_kv* kv, const af_paged_batch* batch, void* k_out, void* v_out,
+                                      void* stream) {
+    Paged p;
+    const af_status st = paged_args(kv, batch, &p);
+    if (st != AF_OK) return st;
+    if (p.n_seqs == 0 || p.n_tokens == 0) return AF_OK;
+    if (k_out == nullptr || v_out == nullptr || !aligned(k_out, 16) || !aligned(v_out, 16)) return AF_ERR_INVALID;
+    cudaError_t e;
+    unsigned* fault = paged_fault_word(&e);
+    if (fault == nullptr) return cuda_fail(e, "af_paged_kv_read");
+    const unsigned grid = (unsigned)(((long long)p.n_tokens + kReadRows - 1) / kReadRows);
+    paged_dispatch(kv, [&](auto fmt, auto hd) {
+        paged_read_kernel<decltype(fmt)::value, decltype(hd)::value>
+            <<<grid, kReadThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+                p, static_cast<__half*>(k_out), static_cast<__half*>(v_out), fault);
+    });
+    e = cudaGetLastError();
+    return e == cudaSuccess ? AF_OK : cuda_fail(e, "paged_read_kernel");
+}
+
+extern "C" af_status af_paged_attention(const af_paged_kv* kv, const af_paged_batch* batch, const void* q,
+                                        int64_t q_stride, int n_heads, float scale, int max_rows, int max_kv,
+                                        void* out, void* stream) {
+    Paged p;
+    const af_status st = paged_args(kv, batch, &p);
+    if (st != AF_OK) return st;
+    if (n_heads < 1 || n_heads > 65535 || n_heads % p.NKV != 0) return AF_ERR_INVALID;
+    if (q_stride < (int64_t)n_heads * kv->head_dim || q_stride % 8 != 0) return AF_ERR_INVALID;
+    if (!(scale > 0.f) || !std::isfinite(scale) || max_rows < 0 || max_kv < 0) return AF_ERR_INVALID;
+    if (p.n_seqs == 0 || p.n_tokens == 0) return AF_OK;
+    if (q == nullptr || out == nullptr || !aligned(q, 16) || !aligned(out, 16)) return AF_ERR_INVALID;
+    cudaError_t e;
+    unsigned* fault = paged_fault_word(&e);
+    if (fault == nullptr) return cuda_fail(e, "af_paged_attention");
+    paged_dispatch(kv, [&](auto fmt, auto hd) {
+        paged_attention_kernel<decltype(fmt)::value, decltype(hd)::value>
+            <<<dim3(p.n_tokens, (n_heads + kAttnWarps - 1) / kAttnWarps), kAttnWarps * 32, 0,
+               static_cast<cudaStream_t>(stream)>>>(p, static_cast<const __half*>(q), q_stride,
+                                                    static_cast<__half*>(out), n_heads, scale, fault);
+    });
+    e = cudaGetLastError();
+    return e == cudaSuccess ? AF_OK : cuda_fail(e, "paged_attention_kernel");
+}

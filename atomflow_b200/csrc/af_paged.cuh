@@ -1,0 +1,151 @@
+// af_paged.cuh -- what the kernels over a paged KV cache share: the cache and the
+// batch as they see them, the checks that keep every access inside the pool
+// whatever the device arrays hold, and the cache formats' codes.
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <cmath>
+#include <cstdint>
+
+#include "af_common.cuh"
+#include "af_internal.h"
+
+namespace af {
+
+constexpr int kPagedMinPage = 8, kPagedMaxPage = 256;
+
+// The cache and the batch, by value, as a kernel argument.
+struct Paged {
+    uint8_t *k, *v;              // pages [n_pages][page][NKV][HD]
+    __half *ks, *vs;             // scales [n_pages][page][NKV] (8-bit formats)
+    long long page_bytes;        // from one page to the next
+    long long scale_stride;      // scales from one page to the next
+    const int *cu, *len, *table;
+    long long table_stride;
+    int n_pages, page_shift, NKV;
+    int n_seqs, n_tokens, max_pages;
+};
+
+// Fault bits of the paged operators (af_paged.cu), through a pointer: the
+// kernels live in several translation units.
+unsigned* paged_fault_word(cudaError_t* err);
+
+// One sequence: its rows [row0, row0 + q) and its cached positions.  A sequence
+// whose offsets or length make no sense (rows outside [0, n_tokens), decreasing
+// offsets, more positions than its table has pages for) counts as empty.
+struct PagedSeq {
+    int row0, q, kv;
+};
+__device__ __forceinline__ PagedSeq paged_seq(const Paged& p, int b, unsigned* fault) {
+    const int s = __ldg(p.cu + b), e = __ldg(p.cu + b + 1), kv = __ldg(p.len + b);
+    if (s < 0 || e < s || e > p.n_tokens || kv < 0 || (long long)kv > ((long long)p.max_pages << p.page_shift)) {
+        atomicOr(fault, (unsigned)AF_FAULT_PAGED);
+        return {0, 0, 0};
+    }
+    return {s, e - s, kv};
+}
+
+// The sequence whose rows hold row t: the last b with cu[b] <= t (empty
+// sequences share their offset with the next one).  Not checked: paged_seq is.
+__device__ __forceinline__ int paged_find(const Paged& p, int t) {
+    int lo = 0, hi = p.n_seqs;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (__ldg(p.cu + mid) <= t) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// Page of position pos of sequence b; -1 (and the fault bit) where the table's
+// entry is not a page of the pool.
+__device__ __forceinline__ int paged_page(const Paged& p, int b, int pos, unsigned* fault) {
+    const int page = __ldg(p.table + (long long)b * p.table_stride + (pos >> p.page_shift));
+    if ((unsigned)page < (unsigned)p.n_pages) return page;
+    atomicOr(fault, (unsigned)AF_FAULT_PAGED);
+    return -1;
+}
+// Index of a position's row of NKV vectors in its page.
+__device__ __forceinline__ int paged_slot(const Paged& p, int pos) { return pos & ((1 << p.page_shift) - 1); }
+
+// ---- formats ----
+template <int FMT>
+struct KvFormat;
+template <>
+struct KvFormat<AF_KV_F16> {
+    static constexpr int kBytes = 2;
+};
+// 8-bit codes: value = code * scale.  kScaleMax is the largest FP16 scale whose
+// product with the largest code is a finite FP16 value.
+template <>
+struct KvFormat<AF_KV_FP8_E4M3> {
+    static constexpr int kBytes = 1;
+    static constexpr float kCodeMax = 448.f, kScaleMax = 146.125f;
+};
+template <>
+struct KvFormat<AF_KV_INT8> {
+    static constexpr int kBytes = 1;
+    static constexpr float kCodeMax = 127.f, kScaleMax = 515.5f;
+};
+
+// Four codes (one word, lowest address first) -> four FP16 values in two words, exactly.
+// E4M3 by the packed conversion.  INT8: byte b ^ 0x80 as the mantissa of 1024
+// gives 1024 + b + 128 exactly; subtracting 1152 leaves b.
+template <int FMT>
+__device__ __forceinline__ void kv_unpack4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    if constexpr (FMT == AF_KV_FP8_E4M3) {
+        lo = e4m3x2_lo(w);
+        hi = e4m3x2_hi(w);
+    } else {
+        w ^= 0x80808080u;
+        const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+        const __half2 off = __float2half2_rn(1152.f);
+        const __half2 ra = __hsub2(*reinterpret_cast<const __half2*>(&a), off);
+        const __half2 rb = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+        lo = *reinterpret_cast<const uint32_t*>(&ra);
+        hi = *reinterpret_cast<const uint32_t*>(&rb);
+    }
+}
+// Two FP16 values times a pair of FP16 scales, one rounding each.
+__device__ __forceinline__ uint32_t mul_half2(uint32_t v, __half2 s) {
+    const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&v), s);
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// The scale of a vector whose largest magnitude is amax: the smallest FP16 value
+// that brings it to at most the largest code (rounded up, so that no element
+// saturates however small the scale), 1 for a vector of zeros.  NaN elements do
+// not count; an infinity takes the largest scale.
+template <int FMT>
+__device__ __forceinline__ __half kv_scale(float amax) {
+    if (amax == 0.f) return __float2half_rn(1.f);
+    const __half s = __float2half_ru(__fdiv_rn(amax, KvFormat<FMT>::kCodeMax));
+    return __hmin(s, __float2half_rn(KvFormat<FMT>::kScaleMax));
+}
+// Four values -> four codes: round to nearest even of x / scale, saturating.
+template <int FMT>
+__device__ __forceinline__ uint32_t kv_pack4(const float (&x)[4], float scale) {
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = __fdiv_rn(x[i], scale);
+    if constexpr (FMT == AF_KV_FP8_E4M3) {
+        const uint32_t a = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t b = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
+        return a | (b << 16);
+    } else {
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c = __float2int_rn(fminf(fmaxf(y[i], -127.f), 127.f));
+            w |= (uint32_t)(y[i] == y[i] ? c & 0xff : 0) << (8 * i);
+        }
+        return w;
+    }
+}
+
+// ---- host side (af_paged.cu) ----
+af_status paged_args(const af_paged_kv* kv, const af_paged_batch* batch, Paged* out);
+
+}  // namespace af

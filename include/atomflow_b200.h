@@ -59,7 +59,8 @@ typedef enum af_fault_bits {
     AF_FAULT_X_COPY = 1,      /* a GEMV's bounded wait for its x copy ran out (that y is invalid) */
     AF_FAULT_POSITION = 2,    /* a decode kernel read a position outside [0, max_seq) and skipped its work */
     AF_FAULT_CHAIN_WAIT = 4,  /* a projection chain's bounded wait ran out (that launch's outputs are invalid) */
-    AF_FAULT_TC_WAIT = 8      /* an af_w8a16_gemm_tc bounded wait ran out (its outputs are invalid) */
+    AF_FAULT_TC_WAIT = 8,     /* a bounded wait of af_w8a16_gemm_tc or af_paged_attention ran out (its outputs are invalid) */
+    AF_FAULT_PAGED = 16       /* a paged operator met offsets, a length or a page outside its arguments' ranges */
 } af_fault_bits;
 
 const char* af_status_string(af_status s);
@@ -313,6 +314,95 @@ af_status af_gemv_chain(const af_chain_op* ops, int n_ops, void* workspace, size
  * its summation order, so not bit-identical to it.  Same arguments. */
 af_status af_gemv_chain_fast(const af_chain_op* ops, int n_ops, void* workspace, size_t workspace_bytes,
                              void* stream);
+
+/* ------------------------------------------------------ paged KV cache ---
+ * A KV cache in pages for a batch of sequences, in FP16 or in 8 bits: the
+ * batched counterparts of af_rope_kv_write and af_decode_attention for prompts
+ * taken in chunks and for many sequences at once.  No counterpart in the
+ * reference (one sequence, one contiguous FP16 cache).
+ *
+ * Pool: k and v hold n_pages pages [page_size][n_kv_heads][head_dim], a page
+ * being a stretch of the same token-major rows as the one-sequence cache.
+ * page_stride is the distance in elements between pages (>= page_size *
+ * n_kv_heads * head_dim, a multiple of 16 bytes; k and v alike), so several
+ * pools may interleave.  8-bit formats keep one FP16 scale per head vector:
+ * scales [page_size][n_kv_heads] per page, scale_stride elements apart.
+ *   AF_KV_F16        the values
+ *   AF_KV_FP8_E4M3   value = half(code * scale), scale = max|x| / 448
+ *   AF_KV_INT8       value = half(code * scale), scale = max|x| / 127
+ * The scale is rounded up to FP16 (no element saturates), is 1 for a vector of
+ * zeros and at most 146.125 / 515.5 (every value stays finite in FP16; an
+ * infinity is stored as the largest code, NaN as E4M3's NaN or INT8's 0).  Codes
+ * are round-to-nearest-even of x / scale.  head_dim is 64 or 128, page_size a
+ * power of two from 8 to 256; k, v 16-byte aligned.
+ *
+ * Batch: sequence b owns rows [cu_rows[b], cu_rows[b+1]) of the call's packed
+ * rows (n_tokens of them in the buffers) and kv_len[b] cached positions; its
+ * row i stands at position kv_len[b] - (cu_rows[b+1] - cu_rows[b]) + i, so
+ * kv_len counts the call's own rows.  block_table [n_seqs][max_pages] (rows
+ * table_stride ints apart) names the page of positions [j * page_size, ...).
+ * All four are device arrays, read when the kernel runs: a captured call
+ * follows their values.  Sequences may share pages, for reading; two rows of one
+ * write that name the same slot leave it with either's data.  Rows of no
+ * sequence (behind the last one) are left as they were.  A row before position
+ * 0 (a chunk longer than kv_len) has nothing to do with the cache: write skips
+ * it, read and attention give zeros.
+ * What the arrays hold cannot lead outside the buffers: a sequence whose rows
+ * leave [0, n_tokens), whose offsets decrease or whose kv_len exceeds its
+ * table is skipped, a page outside [0, n_pages) is written nowhere and read as
+ * zeros, and each sets AF_FAULT_PAGED (af_device_faults).
+ *
+ *   af_paged_kv_write   qkv FP16 [n_tokens] rows [NH*HD | NKV*HD | NKV*HD],
+ *                       qkv_stride elements apart (a multiple of 8), n_heads 0
+ *                       for rows of k and v alone.  With cos_tab / sin_tab
+ *                       (af_rope_tables, max_seq rows): q and k are rotated at
+ *                       the rows' positions, as af_rope_kv_write rotates them,
+ *                       and rounded to FP16; q goes to q_out [n_tokens][NH][HD]
+ *                       (not overlapping qkv), k and v to the pages.  A position
+ *                       outside the tables sets AF_FAULT_POSITION and skips its
+ *                       row.  Tables NULL: k and v are stored as they are, q is
+ *                       left alone (q_out may be NULL).
+ *   af_paged_kv_read    the rows' positions as FP16 k_out, v_out
+ *                       [n_tokens][NKV][HD] (cu_rows = sums of kv_len: whole
+ *                       sequences; fewer rows: each sequence's last ones).
+ *   af_paged_attention  out[row, h] = softmax(scale * q k^T) v over the
+ *                       positions up to the row's own, q FP16 [n_tokens] rows
+ *                       [NH][HD] q_stride elements apart (a multiple of 8), out
+ *                       FP16 [n_tokens][NH][HD], NH % NKV == 0.  max_rows and
+ *                       max_kv are the host's bounds on a sequence's rows and
+ *                       positions (0: not known): they choose how the work is
+ *                       split, never the result's meaning.
+ * q, out, qkv, q_out, k_out, v_out 16-byte aligned.  No workspace; no
+ * allocation. */
+typedef enum af_kv_format {
+    AF_KV_F16 = 0,
+    AF_KV_FP8_E4M3 = 1,
+    AF_KV_INT8 = 2
+} af_kv_format;
+typedef struct af_paged_kv {
+    int format;               /* af_kv_format */
+    int n_pages, page_size, n_kv_heads, head_dim;
+    void* k;
+    void* v;
+    int64_t page_stride;      /* elements */
+    void* k_scale;            /* 8-bit formats; else NULL */
+    void* v_scale;
+    int64_t scale_stride;     /* elements */
+} af_paged_kv;
+typedef struct af_paged_batch {
+    int n_seqs, n_tokens, max_pages;
+    const int* cu_rows;       /* device [n_seqs + 1] */
+    const int* kv_len;        /* device [n_seqs] */
+    const int* block_table;   /* device [n_seqs][max_pages] */
+    int64_t table_stride;     /* ints */
+} af_paged_batch;
+af_status af_paged_kv_write(const af_paged_kv* kv, const af_paged_batch* batch, const void* qkv, int64_t qkv_stride,
+                            int n_heads, const float* cos_tab, const float* sin_tab, int max_seq, void* q_out,
+                            void* stream);
+af_status af_paged_kv_read(const af_paged_kv* kv, const af_paged_batch* batch, void* k_out, void* v_out,
+                           void* stream);
+af_status af_paged_attention(const af_paged_kv* kv, const af_paged_batch* batch, const void* q, int64_t q_stride,
+                             int n_heads, float scale, int max_rows, int max_kv, void* out, void* stream);
 
 /* -------------------------------------------------------- decode engine ---
  * A whole greedy decode step of a model in the reference's .bin format
