@@ -5,6 +5,9 @@
 // The batched, paged counterparts of af_rope_kv_write and af_decode_attention:
 // one page is a stretch of the same token-major rows [NKV * HD] that the
 // one-sequence cache has, so a contiguous cache is a pool whose table counts up.
+#include <algorithm>
+#include <type_traits>
+
 #include "af_paged.cuh"
 
 using namespace af;
@@ -424,12 +427,9 @@ extern "C" af_status af_paged_attention(const af_paged_kv* kv, const af_paged_ba
     cudaError_t e;
     unsigned* fault = paged_fault_word(&e);
     if (fault == nullptr) return cuda_fail(e, "af_paged_attention");
-    paged_dispatch(kv, [&](auto fmt, auto hd) {
-        paged_attention_kernel<decltype(fmt)::value, decltype(hd)::value>
-            <<<dim3(p.n_tokens, (n_heads + kAttnWarps - 1) / kAttnWarps), kAttnWarps * 32, 0,
-               static_cast<cudaStream_t>(stream)>>>(p, static_cast<const __half*>(q), q_stride,
-                                                    static_cast<__half*>(out), n_heads, scale, fault);
-    });
-    e = cudaGetLastError();
+    const long long cap = (long long)p.max_pages << p.page_shift;
+    const int kv_bound = (int)std::min<long long>(max_kv > 0 ? max_kv : cap, cap);
+    e = paged_chunk_launch(kv->format, kv->head_dim, p, q, q_stride, n_heads, scale, 0, kv_bound, out, fault,
+                           static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? AF_OK : cuda_fail(e, "paged_attention_kernel");
 }

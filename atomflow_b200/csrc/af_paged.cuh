@@ -147,5 +147,9 @@ __device__ __forceinline__ uint32_t kv_pack4(const float (&x)[4], float scale) {
 
 // ---- host side (af_paged.cu) ----
 af_status paged_args(const af_paged_kv* kv, const af_paged_batch* batch, Paged* out);
+// The tensor-core attention (af_paged_tc.cu) over every sequence of more than
+// skip_rows rows (tokens x query heads per kv head).
+cudaError_t paged_chunk_launch(int format, int head_dim, const Paged& p, const void* q, long long q_stride, int n_heads,
+                               float scale, int skip_rows, int max_kv, void* out, unsigned* fault, cudaStream_t st);
 
 }  // namespace af

@@ -1,0 +1,680 @@
+// af_paged_tc.cu -- attention of chunks of new tokens over a paged KV cache on the
+// tcgen05 tensor cores (af_paged_attention's path for more than a few rows per
+// sequence and kv head).
+//
+//   S = Q K^T,  P = exp2(c S - c m),  O = sum over tiles of P V,  out = O / l
+//
+// c = scale * log2(e), m the row's running maximum, l the running sum of P.
+//
+//   * Rows: the G query heads that share a kv head see the same K and V, so the
+//     rows of a work item are (token, head of the group) pairs of one sequence,
+//     256 of them: two 128-row MMA tiles that share every K and V tile read.
+//   * Warps 12-15 load: K and V tiles of 128 positions, row by row through the
+//     block table (16-byte cp.async for FP16; 8-bit codes pass through registers
+//     and are multiplied by their scale into FP16, the values af_paged_kv_read
+//     returns), into a ring of slots in the 128-byte-swizzled layout that the
+//     MMA reads.  Positions at or past the sequence's end are zeros.
+//   * Warp 8 issues the MMAs.  S of both row tiles and O of both fill the 512
+//     TMEM columns; P (FP16) overwrites the S it came from and is the A operand
+//     of the second product straight from TMEM.  The order PV(0, j), QK(0, j+1),
+//     PV(1, j), QK(1, j+1) keeps the tensor core on one row tile while the other
+//     is in its softmax.
+//   * Warps 0-3 and 4-7 are the softmax of row tile 0 and 1, one row per thread:
+//     no shuffles.  O is rescaled only when the row's maximum has grown by more
+//     than a factor 2^8 since the last rescale (P then stays below 2^8, exact
+//     range in FP16; l and O are FP32), which ends after the first few tiles.
+//   * P is rounded to FP16 for the second product: its error, 2^-12 of each
+//     weight on average, is that of the FP16 output's own rounding.
+//   * Few rows and a long cache: a work item's positions are split over the CTAs
+//     of a cluster, which merge through distributed shared memory in rank order
+//     -- no workspace, no second launch, the same bits every time.
+//   * Every wait is bounded; one that runs out sets AF_FAULT_TC_WAIT and the
+//     kernel ends without waiting further.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
+#include "af_paged.cuh"
+
+namespace af {
+namespace {
+
+constexpr int kTile = 128;              // rows of an MMA tile; positions of a K or V tile
+constexpr int kItemRows = 2 * kTile;
+constexpr int kThreads = 512;
+constexpr int kLoadWarp = 12, kMmaWarp = 8;
+constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr int kMaxSplit = 8;
+constexpr float kGrow = 8.f;            // log2 of the growth of the maximum that forces a rescale
+constexpr int kTmemCols = 512;
+
+template <int HD>
+struct Shape {
+    static constexpr int kTileBytes = kTile * HD * 2;    // one 128 x HD FP16 tile
+    static constexpr int kSlots = HD == 128 ? 5 : 8;
+    static constexpr int kQBytes = 2 * kTileBytes;
+    static constexpr size_t kSmem = kQBytes + (size_t)kSlots * kTileBytes + 1024;   // + alignment to 1 KB
+};
+static_assert(Shape<128>::kSmem + 512 <= 227 * 1024, "shared memory");
+
+struct TcArgs {
+    const __half* q;
+    long long q_stride;
+    __half* out;
+    int NH, G;
+    float c;            // scale * log2(e)
+    int skip_rows;      // sequences of at most this many rows (tokens x G) belong to another kernel
+};
+
+// ---- tcgen05 (PTX ISA) ----
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_alloc(uint32_t dst, uint32_t ncols) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(ncols)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_relinquish() {
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// D[tmem] (+)= A[smem] B[smem]
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// D[tmem] (+)= A[tmem] B[smem]
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// 16 or 32 consecutive 32-bit TMEM columns of this warp's 32 lanes -> registers and back.  Loaded values are there
+// only after tmem_wait_ld; tmem_pin keeps their uses behind it.
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_pin(uint32_t (&r)[16]) {
+    asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
+}
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_pin(uint32_t (&r)[32]) {
+    asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
+}
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+// Shared-memory matrix descriptor, 128-byte swizzle (layout type 2 at bits 61-63), version 1.  K-major (Q, K):
+// sbo = bytes between 8-row groups.  N-major (V): lbo = bytes between 64-element panels, sbo = between 8-position
+// groups.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) |
+           ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// kind::f16 instruction descriptor: FP32 accumulator, FP16 operands, A K-major, M = 128.
+__device__ __forceinline__ constexpr uint32_t instr_desc(int n, bool b_n_major) {
+    return (1u << 4) | (b_n_major ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+}
+__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, uint32_t n) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// (a, b) * (m, m) + (k, k) in one packed FP32 FMA
+__device__ __forceinline__ void fma2(float& a, float& b, float m, float k) {
+    unsigned long long x, mm, kk;
+    asm("mov.b64 %0, {%1,%2};" : "=l"(x) : "f"(a), "f"(b));
+    asm("mov.b64 %0, {%1,%1};" : "=l"(mm) : "f"(m));
+    asm("mov.b64 %0, {%1,%1};" : "=l"(kk) : "f"(k));
+    asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(x) : "l"(mm), "l"(kk));
+    asm("mov.b64 {%0,%1}, %2;" : "=f"(a), "=f"(b) : "l"(x));
+}
+__device__ __forceinline__ void add2(float& a, float& b, float c, float d) {
+    unsigned long long x, y;
+    asm("mov.b64 %0, {%1,%2};" : "=l"(x) : "f"(a), "f"(b));
+    asm("mov.b64 %0, {%1,%2};" : "=l"(y) : "f"(c), "f"(d));
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(y));
+    asm("mov.b64 {%0,%1}, %2;" : "=f"(a), "=f"(b) : "l"(x));
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+struct Bars {
+    uint64_t full[8], empty[8];    // ring slots
+    uint64_t s_full[2], p_full[2]; // per row tile
+    uint64_t o_done;
+};
+
+// Bounded wait: false once the limit has passed (the fault bit is set).
+__device__ __forceinline__ bool tc_wait(const uint64_t* bar, uint32_t parity, volatile int* abort, unsigned* fault) {
+    const uint32_t b = smem_u32(bar);
+    if (mbar_try_wait(b, parity)) return true;
+    if (*abort) return false;
+    if (mbar_wait_bounded(b, parity, kWaitNs)) return true;
+    atomicOr(fault, (unsigned)AF_FAULT_TC_WAIT);
+    *abort = 1;
+    return false;
+}
+
+template <int FMT, int HD>
+__global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p, const TcArgs a, unsigned* fault) {
+    namespace cg = cooperative_groups;
+    using Sh = Shape<HD>;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) Bars bars;
+    __shared__ uint32_t s_tmem;
+    __shared__ volatile int s_abort;
+    __shared__ int s_item[2];                        // sequence, row tile pair
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int S = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int cid = blockIdx.x / S, kvh = cid % p.NKV, item = cid / p.NKV;
+
+    // ------------------------------------------------ which work item is ours
+    if (warp == 0) {
+        int seen = 0, fb = -1, ft = 0;
+        for (int b0 = 0; b0 < p.n_seqs && fb < 0; b0 += 32) {
+            const int b = b0 + lane;
+            int n = 0;
+            if (b < p.n_seqs) {
+                const PagedSeq s = paged_seq(p, b, fault);
+                const long long rows = (long long)s.q * a.G;
+                n = rows > a.skip_rows ? (int)((rows + kItemRows - 1) / kItemRows) : 0;
+            }
+            int inc = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += u;
+            }
+            const bool mine = item >= seen + inc - n && item < seen + inc;
+            const unsigned who = __ballot_sync(0xffffffffu, mine);
+            if (who) {
+                const int src = __ffs(who) - 1;
+                fb = b0 + src;
+                // later rows see more positions: they go first
+                ft = __shfl_sync(0xffffffffu, seen + inc - 1 - item, src);
+            }
+            seen += __shfl_sync(0xffffffffu, inc, 31);
+        }
+        if (lane == 0) {
+            s_item[0] = fb;
+            s_item[1] = ft;
+            s_abort = 0;
+        }
+    }
+    if (warp == kMmaWarp) {
+        tmem_alloc(smem_u32(&s_tmem), kTmemCols);
+        tmem_relinquish();
+    }
+    if (threadIdx.x == 32) {
+        for (int i = 0; i < 8; ++i) {
+            mbar_init(smem_u32(&bars.full[i]), 128);
+            mbar_init(smem_u32(&bars.empty[i]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&bars.s_full[i]), 1);
+            mbar_init(smem_u32(&bars.p_full[i]), 128);
+        }
+        mbar_init(smem_u32(&bars.o_done), 1);
+        mbar_init_fence();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    const int b = s_item[0];
+    if (b < 0) {   // no such item: the whole cluster leaves
+        if (warp == kMmaWarp) tmem_dealloc(tmem, kTmemCols);
+        return;
+    }
+    const PagedSeq seq = paged_seq(p, b, fault);
+    const int row_base = s_item[1] * kItemRows;
+    const int rows = min(kItemRows, (int)min((long long)seq.q * a.G - row_base, (long long)kItemRows));
+    const int n_sub = rows > kTile ? 2 : 1;          // row tiles in use
+    const int ctx = seq.kv - seq.q;
+    const int last_token = (row_base + rows - 1) / a.G;
+    const int end = max(0, ctx + last_token + 1);    // positions any row sees
+    const int tiles = (end + kTile - 1) / kTile;
+    const int t0 = (int)((long long)tiles * rank / S), t1 = (int)((long long)tiles * (rank + 1) / S);
+    const int n = t1 - t0;
+    unsigned char* q_s = smem;
+    unsigned char* ring = smem + Sh::kQBytes;
+    // the cluster merge's parts, in the buffers once they are idle: FP32 O [256][HD], then m and l [256]
+    float* part_o = reinterpret_cast<float*>(smem);
+    float* part_m = part_o + kItemRows * HD;
+    float* part_l = part_m + kItemRows;
+    static_assert((kItemRows * HD + 2 * kItemRows) * 4 <= Sh::kSmem - 1024, "parts fit");
+
+    if (warp >= kLoadWarp) {
+        // ------------------------------------------------------------- loaders
+        // registers are handed over once, here, and never taken back: 2 x 184 + 48 + 96 = 4 x 128
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+        const int i = threadIdx.x - kLoadWarp * 32;
+        constexpr int CH = HD / 8;                   // 16-byte FP16 chunks of a row
+        if (n > 0) {
+            const int c = i % CH, r0 = i / CH;
+            constexpr int RS = 128 / CH;             // rows between a thread's rows (a multiple of 8)
+            const uint32_t at = smem_u32(q_s) + (c >> 3) * (kTile * 128) + r0 * 128 + (((c & 7) ^ (r0 & 7)) << 4);
+#pragma unroll 4
+            for (int k = 0; k < kItemRows / RS; ++k) {
+                const int r = r0 + k * RS;
+                const int R = row_base + r, tok = R / a.G, hd = R - tok * a.G;
+                const bool ok = r < rows;
+                const __half* src = a.q + (ok ? (long long)(seq.row0 + tok) * a.q_stride + (kvh * a.G + hd) * HD + c * 8 : 0);
+                const int rt = k * RS;               // r0 < RS: the tile is that of k * RS
+                cp_async16_zfill(at + (rt >> 7) * Sh::kTileBytes + (rt & 127) * 128, src, ok ? 16u : 0u);
+            }
+            cp_async_commit();
+        }
+        if constexpr (FMT == AF_KV_F16) {
+            constexpr int RS = 128 / CH, KR = kTile / RS;   // rows of a tile per thread
+            const int c = i % CH, r0 = i / CH;
+            const uint32_t at = (c >> 3) * (kTile * 128) + r0 * 128 + (((c & 7) ^ (r0 & 7)) << 4);
+            constexpr int D = 2;                            // tiles left in flight behind the newest
+            int pg[KR];
+            for (int m = 0; m < 2 * n + D; ++m) {
+                if (m < 2 * n) {
+                    const int slot = m % Sh::kSlots, j0 = (t0 + (m >> 1)) * kTile;
+                    if (!(m & 1)) {                         // K: look the pages up; V: the same
+#pragma unroll
+                        for (int k = 0; k < KR; ++k) {
+                            const int pos = j0 + r0 + k * RS;
+                            pg[k] = pos < end ? paged_page(p, b, pos, fault) : -1;
+                        }
+                    }
+                    if (m >= Sh::kSlots) tc_wait(&bars.empty[slot], (m / Sh::kSlots - 1) & 1, &s_abort, fault);
+                    const uint8_t* base = (m & 1) ? p.v : p.k;
+                    const uint32_t dst = smem_u32(ring) + slot * Sh::kTileBytes + at;
+#pragma unroll
+                    for (int k = 0; k < KR; ++k) {
+                        const int pos = j0 + r0 + k * RS;
+                        const bool ok = pg[k] >= 0;
+                        const uint8_t* src = base + (ok ? pg[k] * p.page_bytes + ((long long)paged_slot(p, pos) * p.NKV + kvh) * (HD * 2) + c * 16 : 0);
+                        cp_async16_zfill(dst + k * RS * 128, src, ok ? 16u : 0u);
+                    }
+                }
+                cp_async_commit();
+                if (m >= D) {
+                    cp_async_wait<D>();
+                    fence_async_smem();
+                    mbar_arrive(smem_u32(&bars.full[(m - D) % Sh::kSlots]));
+                }
+            }
+            cp_async_wait<0>();
+        } else {   // 8-bit
+            constexpr int C8 = HD / 16;                     // 16-code chunks of a row
+            constexpr int RS = 128 / C8, KR = kTile / RS;
+            const int c = i % C8, r0 = i / C8;
+            // code chunk c makes FP16 chunks 2c and 2c + 1 of panel c / 4
+            const uint32_t row_at = (c >> 2) * (kTile * 128) + r0 * 128;
+            const uint32_t x0 = ((2 * c) & 7) ^ (r0 & 7), x1 = ((2 * c + 1) & 7) ^ (r0 & 7);
+            uint4 code[KR];
+            __half sc[KR];
+            auto fetch = [&](int m) {
+                const int j0 = (t0 + (m >> 1)) * kTile;
+                const uint8_t* base = (m & 1) ? p.v : p.k;
+                const __half* sbase = (m & 1) ? p.vs : p.ks;
+#pragma unroll
+                for (int k = 0; k < KR; ++k) {
+                    const int pos = j0 + r0 + k * RS;
+                    const int page = pos < end ? paged_page(p, b, pos, fault) : -1;
+                    code[k] = make_uint4(0u, 0u, 0u, 0u);
+                    sc[k] = __float2half_rn(0.f);
+                    if (page >= 0) {
+                        const long long slot = (long long)paged_slot(p, pos) * p.NKV + kvh;
+                        code[k] = __ldg(reinterpret_cast<const uint4*>(base + page * p.page_bytes + slot * HD + c * 16));
+                        sc[k] = __ldg(sbase + page * p.scale_stride + slot);
+                    }
+                }
+            };
+            if (n > 0) fetch(0);
+            cp_async_wait<0>();                             // Q
+            for (int m = 0; m < 2 * n; ++m) {
+                const int slot = m % Sh::kSlots;
+                if (m >= Sh::kSlots) tc_wait(&bars.empty[slot], (m / Sh::kSlots - 1) & 1, &s_abort, fault);
+                unsigned char* dst = ring + slot * Sh::kTileBytes + row_at;
+#pragma unroll
+                for (int k = 0; k < KR; ++k) {
+                    const __half2 s2 = __half2half2(sc[k]);
+                    const uint32_t in[4] = {code[k].x, code[k].y, code[k].z, code[k].w};
+                    uint32_t o[8];
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        kv_unpack4<FMT>(in[w], o[2 * w], o[2 * w + 1]);
+                        o[2 * w] = mul_half2(o[2 * w], s2);
+                        o[2 * w + 1] = mul_half2(o[2 * w + 1], s2);
+                    }
+                    *reinterpret_cast<uint4*>(dst + k * RS * 128 + x0 * 16) = make_uint4(o[0], o[1], o[2], o[3]);
+                    *reinterpret_cast<uint4*>(dst + k * RS * 128 + x1 * 16) = make_uint4(o[4], o[5], o[6], o[7]);
+                }
+                fence_async_smem();
+                mbar_arrive(smem_u32(&bars.full[slot]));
+                if (m + 1 < 2 * n) fetch(m + 1);
+            }
+        }
+    } else if (warp >= kMmaWarp) {
+        // ----------------------------------------------------------- MMA issue
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        if (warp == kMmaWarp) {
+            constexpr uint32_t qk_desc = instr_desc(kTile, false), pv_desc = instr_desc(HD, true);
+            const uint32_t q0 = smem_u32(q_s), r0 = smem_u32(ring);
+            auto qk = [&](int i, int m) {   // S_i = Q_i K^T with the K tile of ring entry m
+                const uint32_t k0 = r0 + (m % Sh::kSlots) * Sh::kTileBytes;
+#pragma unroll
+                for (int s = 0; s < HD / 16; ++s) {
+                    const uint32_t off = (s >> 2) * (kTile * 128) + (s & 3) * 32;
+                    mma_ss(tmem + i * kTile, smem_desc(q0 + i * Sh::kTileBytes + off, 16, 1024),
+                           smem_desc(k0 + off, 16, 1024), qk_desc, s > 0);
+                }
+                tc_commit(smem_u32(&bars.s_full[i]));
+            };
+            auto pv = [&](int i, int m, bool acc) {   // O_i (+)= P_i V
+                const uint32_t v0 = r0 + (m % Sh::kSlots) * Sh::kTileBytes;
+#pragma unroll
+                for (int s = 0; s < kTile / 16; ++s)
+                    mma_ts(tmem + 2 * kTile + i * kTile, tmem + i * kTile + s * 8,
+                           smem_desc(v0 + s * 2048, kTile * 128, 1024), pv_desc, acc || s > 0);
+            };
+            auto full = [&](int m) {
+                tc_wait(&bars.full[m % Sh::kSlots], (m / Sh::kSlots) & 1, &s_abort, fault);
+                tc_fence_after();
+            };
+            if (n > 0) {
+                full(0);
+                if (lane == 0 && !s_abort) {
+                    for (int i = 0; i < n_sub; ++i) qk(i, 0);
+                    tc_commit(smem_u32(&bars.empty[0]));
+                }
+                __syncwarp();
+                for (int j = 0; j < n; ++j) {
+                    const int mv = 2 * j + 1, mk = 2 * j + 2;
+                    full(mv);
+                    for (int i = 0; i < n_sub; ++i) {
+                        tc_wait(&bars.p_full[i], j & 1, &s_abort, fault);
+                        tc_fence_after();
+                        if (lane == 0 && !s_abort) pv(i, mv, j > 0);
+                        __syncwarp();
+                        if (j + 1 < n) {
+                            if (i == 0) full(mk);
+                            if (lane == 0 && !s_abort) qk(i, mk);
+                            __syncwarp();
+                        }
+                    }
+                    if (lane == 0 && !s_abort) {
+                        tc_commit(smem_u32(&bars.empty[mv % Sh::kSlots]));
+                        if (j + 1 < n) tc_commit(smem_u32(&bars.empty[mk % Sh::kSlots]));
+                        else tc_commit(smem_u32(&bars.o_done));
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+    } else {
+        // ------------------------------------------------------------- softmax
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+        const int i = warp >> 2, r = threadIdx.x & 127;   // row tile, row (= TMEM lane)
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t s_at = tmem + i * kTile + lanes, o_at = tmem + 2 * kTile + i * kTile + lanes;
+        const int R = row_base + i * kTile + r;
+        const bool valid = i * kTile + r < rows;
+        const int tok = R / a.G, head = kvh * a.G + (R - tok * a.G);
+        const int limit = valid ? max(0, ctx + tok + 1) : 0;   // this row sees positions [0, limit)
+        float m = -INFINITY, l0 = 0.f, l1 = 0.f;
+        if (i < n_sub) {
+            for (int j = 0; j < n; ++j) {
+                tc_wait(&bars.s_full[i], j & 1, &s_abort, fault);
+                tc_fence_after();
+                uint32_t v[4][32];
+#pragma unroll
+                for (int h = 0; h < 4; ++h) tmem_ld(s_at + h * 32, v[h]);
+                tmem_wait_ld();
+#pragma unroll
+                for (int h = 0; h < 4; ++h) tmem_pin(v[h]);
+                const int lim = limit - (t0 + j) * kTile;      // of this tile
+                if (__any_sync(0xffffffffu, lim < kTile)) {
+#pragma unroll
+                    for (int h = 0; h < 4; ++h)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (h * 32 + e >= lim) v[h][e] = __float_as_uint(-INFINITY);
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) mx[h] = fmaxf(mx[h], __uint_as_float(v[h][e]));
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                // grow: the old sums are too large a scale off (or there is no scale yet)
+                const bool grow = top > m && !((top - m) * a.c <= kGrow);
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float f = grow ? (m == -INFINITY ? 0.f : ex2((m - top) * a.c)) : 1.f;
+                    if (grow) m = top;
+                    l0 *= f;
+                    l1 *= f;
+                    if (j > 0) {   // the products so far are in O: s_full follows them
+#pragma unroll
+                        for (int h = 0; h < HD / 16; ++h) {
+                            uint32_t o[16];
+                            tmem_ld(o_at + h * 16, o);
+                            tmem_wait_ld();
+                            tmem_pin(o);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tmem_st(o_at + h * 16, o);
+                        }
+                    }
+                }
+                const float k = m == -INFINITY ? 0.f : -m * a.c;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        float x = __uint_as_float(v[2 * h + (e >> 4)][(2 * e) & 31]);
+                        float y = __uint_as_float(v[2 * h + (e >> 4)][(2 * e + 1) & 31]);
+                        fma2(x, y, a.c, k);
+                        x = ex2(x);
+                        y = ex2(y);
+                        add2(l0, l1, x, y);
+                        w[e] = pack_half2(x, y);
+                    }
+                    tmem_st(s_at + h * 32, w);
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(smem_u32(&bars.p_full[i]));
+            }
+            const float l = l0 + l1;
+            if (n > 0) {
+                tc_wait(&bars.o_done, 0, &s_abort, fault);
+                tc_fence_after();
+            }
+            if (S == 1) {
+                const float inv = l > 0.f ? 1.f / l : 0.f;
+                __half* dst = a.out + (long long)(seq.row0 + tok) * a.NH * HD + head * HD;
+#pragma unroll
+                for (int h = 0; h < HD / 32; ++h) {
+                    uint32_t o[32];
+                    if (n > 0) {
+                        tmem_ld(o_at + h * 32, o);
+                        tmem_wait_ld();
+                        tmem_pin(o);
+                    }
+                    if (valid) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int x = 0; x < 4; ++x)
+                                w[x] = n > 0 ? pack_half2(__uint_as_float(o[8 * e + 2 * x]) * inv,
+                                                          __uint_as_float(o[8 * e + 2 * x + 1]) * inv)
+                                             : 0u;
+                            reinterpret_cast<uint4*>(dst + h * 32)[e] = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    }
+                    __syncwarp();
+                }
+            } else {
+                // this CTA's part of the rows: 16-byte chunks
+                // xor the row so that the lanes' stores spread over the banks
+                part_m[i * kTile + r] = m;
+                part_l[i * kTile + r] = l;
+                float4* part = reinterpret_cast<float4*>(part_o) + (size_t)(i * kTile + r) * (HD / 4);
+#pragma unroll
+                for (int h = 0; h < HD / 32; ++h) {
+                    uint32_t o[32];
+                    if (n > 0) {
+                        tmem_ld(o_at + h * 32, o);
+                        tmem_wait_ld();
+                        tmem_pin(o);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = 0u;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        part[(h * 8 + e) ^ (r & (HD / 4 - 1))] =
+                            make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
+                                        __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) tmem_dealloc(tmem, kTmemCols);
+    if (S > 1) {
+        cluster.sync();   // every CTA's part is there
+        // the softmax warps merge: they hold the registers
+        const int sub_rows = n_sub * kTile;
+        const int lo = sub_rows * rank / S, cnt = sub_rows * (rank + 1) / S - lo;
+        for (int x = threadIdx.x; warp < kMmaWarp && x < cnt * (HD / 4); x += kMmaWarp * 32) {
+            const int r = lo + x / (HD / 4), ch = x % (HD / 4);
+            if (r >= rows) break;
+            float M = -INFINITY;
+            for (int u = 0; u < S; ++u) M = fmaxf(M, cluster.map_shared_rank(part_m, u)[r]);
+            float l = 0.f;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int u = 0; u < S; ++u) {   // rank order: the same bits every time
+                const float mu = cluster.map_shared_rank(part_m, u)[r];
+                if (mu == -INFINITY) continue;   // nothing seen there
+                const float f = ex2((mu - M) * a.c);
+                l = fmaf(cluster.map_shared_rank(part_l, u)[r], f, l);
+                const float4 q = reinterpret_cast<const float4*>(cluster.map_shared_rank(part_o, u))[(size_t)r * (HD / 4) + (ch ^ (r & (HD / 4 - 1)))];
+                o.x = fmaf(q.x, f, o.x);
+                o.y = fmaf(q.y, f, o.y);
+                o.z = fmaf(q.z, f, o.z);
+                o.w = fmaf(q.w, f, o.w);
+            }
+            const float inv = l > 0.f ? 1.f / l : 0.f;
+            const int R = row_base + r, tok = R / a.G;
+            __half* dst = a.out + (long long)(seq.row0 + tok) * a.NH * HD + (kvh * a.G + R - tok * a.G) * HD + ch * 4;
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack_half2(o.x * inv, o.y * inv), pack_half2(o.z * inv, o.w * inv));
+        }
+        cluster.sync();   // no CTA leaves while another reads its part
+    }
+}
+
+template <int FMT, int HD>
+cudaError_t launch(const Paged& p, const TcArgs& a, unsigned clusters, int S, unsigned* fault, cudaStream_t st) {
+    auto kernel = paged_chunk_kernel<FMT, HD>;
+    static std::atomic<bool> set[kMaxDevices];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= kMaxDevices || !set[dev].load(std::memory_order_acquire)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<HD>::kSmem);
+        if (e != cudaSuccess) return e;
+        if (dev < kMaxDevices) set[dev].store(true, std::memory_order_release);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(clusters * S);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Shape<HD>::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = S;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, p, a, fault);
+}
+
+}  // namespace
+
+// Launches the chunk kernel over every sequence of more than skip_rows rows.
+cudaError_t paged_chunk_launch(int format, int head_dim, const Paged& p, const void* q, long long q_stride, int n_heads,
+                               float scale, int skip_rows, int max_kv, void* out, unsigned* fault, cudaStream_t st) {
+    TcArgs a{};
+    a.q = static_cast<const __half*>(q);
+    a.q_stride = q_stride;
+    a.out = static_cast<__half*>(out);
+    a.NH = n_heads;
+    a.G = n_heads / p.NKV;
+    a.c = scale * 1.4426950408889634f;
+    a.skip_rows = skip_rows;
+    const long long rows = (long long)p.n_tokens * a.G;
+    // row tile pairs at most: each sequence ends one early, and has more than skip_rows rows
+    const long long seqs = std::min<long long>(p.n_seqs, rows / (skip_rows + 1));
+    const long long items = rows / kItemRows + seqs;
+    const long long clusters = items * p.NKV;
+    if (items == 0) return cudaSuccess;
+    const int sms = device_sm_count();
+    // split an item's positions while the GPU has idle SMs and each CTA keeps four tiles
+    const long long full_items = std::max((rows + kItemRows - 1) / kItemRows, seqs) * p.NKV;
+    int S = 1;
+    while (S < kMaxSplit && full_items * S * 2 <= sms && (long long)max_kv >= (long long)S * 2 * 4 * kTile) S *= 2;
+    if (clusters * S > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+    auto go = [&](auto fmt) {
+        return head_dim == 128 ? launch<decltype(fmt)::value, 128>(p, a, (unsigned)clusters, S, fault, st)
+                               : launch<decltype(fmt)::value, 64>(p, a, (unsigned)clusters, S, fault, st);
+    };
+    if (format == AF_KV_F16) return go(std::integral_constant<int, AF_KV_F16>());
+    if (format == AF_KV_FP8_E4M3) return go(std::integral_constant<int, AF_KV_FP8_E4M3>());
+    return go(std::integral_constant<int, AF_KV_INT8>());
+}
+
+}  // namespace af
