@@ -218,66 +218,6 @@ __global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const Paged p,
     }
 }
 
-// ------------------------------------------------------------ attention
-// One warp per (token, query head): online softmax over the positions it sees,
-// HD / 32 dims per lane.
-constexpr int kAttnWarps = 4;
-
-template <int FMT, int HD>
-__global__ void __launch_bounds__(kAttnWarps * 32) paged_attention_kernel(const Paged p, const __half* __restrict__ q,
-                                                                          long long q_stride, __half* __restrict__ out,
-                                                                          int NH, float scale, unsigned* fault) {
-    constexpr int E = HD / 32;
-    const int t = blockIdx.x, lane = threadIdx.x & 31, h = blockIdx.y * kAttnWarps + (threadIdx.x >> 5);
-    if (h >= NH) return;
-    const int kvh = h / (NH / p.NKV);
-    const int b = paged_find(p, t);
-    const PagedSeq s = paged_seq(p, b, fault);
-    if (t < s.row0 || t >= s.row0 + s.q) return;
-    const int end = s.kv - s.q + (t - s.row0) + 1;
-    float qv[E], o[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        qv[e] = __half2float(q[(long long)t * q_stride + h * HD + lane * E + e]) * scale;
-        o[e] = 0.f;
-    }
-    for (int j = 0; j < end; ++j) {
-        const int page = paged_page(p, b, j, fault);
-        const long long slot = (long long)paged_slot(p, j) * p.NKV + kvh;
-        float k[E], v[E];
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-            float* x = w ? v : k;
-            const uint8_t* src = (w ? p.v : p.k) + (long long)page * p.page_bytes +
-                                 (slot * HD + lane * E) * KvFormat<FMT>::kBytes;
-            float sc = 1.f;
-            if constexpr (FMT != AF_KV_F16)
-                if (page >= 0) sc = __half2float((w ? p.vs : p.ks)[(long long)page * p.scale_stride + slot]);
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                x[e] = 0.f;
-                if (page < 0) continue;
-                if constexpr (FMT == AF_KV_F16) x[e] = __half2float(reinterpret_cast<const __half*>(src)[e]);
-                else if constexpr (FMT == AF_KV_INT8) x[e] = (float)reinterpret_cast<const int8_t*>(src)[e] * sc;
-                else x[e] = (float)reinterpret_cast<const __nv_fp8_e4m3*>(src)[e] * sc;
-            }
-        }
-        float d = 0.f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) d = fmaf(qv[e], k[e], d);
-#pragma unroll
-        for (int x = 16; x > 0; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
-        const float mn = fmaxf(m, d), corr = __expf(m - mn), w = __expf(d - mn);
-        l = fmaf(l, corr, w);
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = fmaf(w, v[e], o[e] * corr);
-        m = mn;
-    }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) out[((long long)t * NH + h) * HD + lane * E + e] = __float2half_rn(o[e] * inv);
-}
-
 }  // namespace
 
 namespace af {
@@ -429,7 +369,19 @@ extern "C" af_status af_paged_attention(const af_paged_kv* kv, const af_paged_ba
     if (fault == nullptr) return cuda_fail(e, "af_paged_attention");
     const long long cap = (long long)p.max_pages << p.page_shift;
     const int kv_bound = (int)std::min<long long>(max_kv > 0 ? max_kv : cap, cap);
-    e = paged_chunk_launch(kv->format, kv->head_dim, p, q, q_stride, n_heads, scale, 0, kv_bound, out, fault,
-                           static_cast<cudaStream_t>(stream));
-    return e == cudaSuccess ? AF_OK : cuda_fail(e, "paged_attention_kernel");
+    // Which kernel takes which sequences is a matter of their rows (new tokens x query heads per kv head), which only
+    // the device knows; the host's bound says which kernels can have work.
+    const cudaStream_t cs = static_cast<cudaStream_t>(stream);
+    const int q_bound = max_rows > 0 ? std::min(max_rows, p.n_tokens) : p.n_tokens;
+    const long long rows_bound = (long long)q_bound * (n_heads / p.NKV);
+    const bool few = rows_bound <= kFewRows;
+    // every sequence as long as the bound: none is short
+    const bool even = (long long)q_bound * p.n_seqs <= p.n_tokens;
+    if (few || !even)
+        e = paged_few_launch(kv->format, kv->head_dim, p, q, q_stride, n_heads, scale, few ? (int)rows_bound : kFewRows,
+                             few, kv_bound, out, fault, cs);
+    if (!few && e == cudaSuccess)
+        e = paged_chunk_launch(kv->format, kv->head_dim, p, q, q_stride, n_heads, scale, even ? 0 : kFewRows, kv_bound,
+                               out, fault, cs);
+    return e == cudaSuccess ? AF_OK : cuda_fail(e, "af_paged_attention");
 }
