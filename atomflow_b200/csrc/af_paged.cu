@@ -6,6 +6,7 @@
 // one page is a stretch of the same token-major rows [NKV * HD] that the
 // one-sequence cache has, so a contiguous cache is a pool whose table counts up.
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "af_paged.cuh"
@@ -63,8 +64,8 @@ __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const Paged 
     load(first + grp);
     const int b = paged_find(p, t);
     const PagedSeq s = paged_seq(p, b, fault);
-    const int pos = s.kv - s.q + (t - s.row0);
-    if (t < s.row0 || t >= s.row0 + s.q || pos < 0) return;   // no sequence's row, or before position 0
+    const int pos = paged_pos_of(s, t);
+    if (pos < 0) return;   // no sequence's row, or before position 0
     if (rotate && pos >= a.max_seq) {
         if (threadIdx.x == 0) atomicOr(fault, (unsigned)AF_FAULT_POSITION);
         return;
@@ -100,9 +101,7 @@ __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const Paged 
                 }
             }
             const int h = v - a.NH - (is_v ? p.NKV : 0);   // kv head; negative for q
-            const long long slot = (long long)paged_slot(p, pos) * p.NKV + h;
-            uint8_t* dst = (is_v ? p.v : p.k) + (long long)page * p.page_bytes +
-                           slot * (HD * KvFormat<FMT>::kBytes);
+            uint8_t* dst = (is_v ? p.v : p.k) + (h < 0 ? 0 : paged_at(p, page, pos, h, HD * KvFormat<FMT>::kBytes));
             if constexpr (FMT == AF_KV_F16) {
                 if (on) {
                     __half* out = v < a.NH ? a.q_out + ((long long)t * a.NH + v) * HD : reinterpret_cast<__half*>(dst);
@@ -135,7 +134,7 @@ __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const Paged 
                     const float f = __half2float(sc);
                     *reinterpret_cast<uint32_t*>(dst + 4 * l) = kv_pack4<FMT>(x, f);
                     *reinterpret_cast<uint32_t*>(dst + HALF + 4 * l) = kv_pack4<FMT>(y, f);
-                    if (l == 0) (is_v ? p.vs : p.ks)[(long long)page * p.scale_stride + slot] = sc;
+                    if (l == 0) (is_v ? p.vs : p.ks)[paged_scale(p, page, pos, h)] = sc;
                 }
             }
         }
@@ -161,10 +160,10 @@ __global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const Paged p,
         if (t < p.n_tokens) {
             const int b = paged_find(p, t);
             const PagedSeq s = paged_seq(p, b, fault);
-            if (t >= s.row0 && t < s.row0 + s.q) {
-                const int pos = s.kv - s.q + (t - s.row0);
+            const int pos = paged_pos_of(s, t);
+            if (pos > INT_MIN) {
                 const int page = pos < 0 ? -1 : paged_page(p, b, pos, fault);
-                at = page < 0 ? -1 : ((long long)page << 32) | paged_slot(p, pos);
+                at = page < 0 ? -1 : ((long long)page << 32) | paged_slot_of(pos, p.page_shift);
             }
         }
         s_at[threadIdx.x] = at;
@@ -186,10 +185,9 @@ __global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const Paged p,
             const bool is_v = w >= pieces;
             const long long at = s_at[r];
             if (at < 0) continue;
-            const long long page = at >> 32, slot = at & 0xffffffff;
-            x[j] = ldg_stream((is_v ? p.v : p.k) + page * p.page_bytes + (slot * pieces + piece) * 16);
-            if constexpr (FMT != AF_KV_F16)
-                sc[j] = __ldg((is_v ? p.vs : p.ks) + page * p.scale_stride + slot * p.NKV + piece / PER);
+            const int page = (int)(at >> 32), slot = (int)(at & 0xffffffff);
+            x[j] = ldg_stream((is_v ? p.v : p.k) + paged_at(p, page, slot, 0, HD * KvFormat<FMT>::kBytes) + piece * 16);
+            if constexpr (FMT != AF_KV_F16) sc[j] = __ldg((is_v ? p.vs : p.ks) + paged_scale(p, page, slot, piece / PER));
         }
 #pragma unroll
         for (int j = 0; j < kReadBatch; ++j) {

@@ -11,6 +11,7 @@
 
 #include "af_common.cuh"
 #include "af_internal.h"
+#include "af_paged_index.h"
 
 namespace af {
 
@@ -32,19 +33,12 @@ struct Paged {
 // kernels live in several translation units.
 unsigned* paged_fault_word(cudaError_t* err);
 
-// One sequence: its rows [row0, row0 + q) and its cached positions.  A sequence
-// whose offsets or length make no sense (rows outside [0, n_tokens), decreasing
-// offsets, more positions than its table has pages for) counts as empty.
-struct PagedSeq {
-    int row0, q, kv;
-};
+// Sequence b; a bad one sets the fault bit and has no rows.
 __device__ __forceinline__ PagedSeq paged_seq(const Paged& p, int b, unsigned* fault) {
-    const int s = __ldg(p.cu + b), e = __ldg(p.cu + b + 1), kv = __ldg(p.len + b);
-    if (s < 0 || e < s || e > p.n_tokens || kv < 0 || (long long)kv > ((long long)p.max_pages << p.page_shift)) {
-        atomicOr(fault, (unsigned)AF_FAULT_PAGED);
-        return {0, 0, 0};
-    }
-    return {s, e - s, kv};
+    const PagedSeq s = paged_seq_of(__ldg(p.cu + b), __ldg(p.cu + b + 1), __ldg(p.len + b), p.n_tokens, p.max_pages,
+                                    p.page_shift);
+    if (s.bad) atomicOr(fault, (unsigned)AF_FAULT_PAGED);
+    return s;
 }
 
 // The sequence whose rows hold row t: the last b with cu[b] <= t (empty
@@ -62,13 +56,18 @@ __device__ __forceinline__ int paged_find(const Paged& p, int t) {
 // Page of position pos of sequence b; -1 (and the fault bit) where the table's
 // entry is not a page of the pool.
 __device__ __forceinline__ int paged_page(const Paged& p, int b, int pos, unsigned* fault) {
-    const int page = __ldg(p.table + (long long)b * p.table_stride + (pos >> p.page_shift));
-    if ((unsigned)page < (unsigned)p.n_pages) return page;
+    const int page = __ldg(p.table + paged_table_at(b, p.table_stride, pos, p.page_shift));
+    if (paged_page_ok(page, p.n_pages)) return page;
     atomicOr(fault, (unsigned)AF_FAULT_PAGED);
     return -1;
 }
-// Index of a position's row of NKV vectors in its page.
-__device__ __forceinline__ int paged_slot(const Paged& p, int pos) { return pos & ((1 << p.page_shift) - 1); }
+// Byte offset of a head vector of the pool, index of its scale.
+__device__ __forceinline__ long long paged_at(const Paged& p, int page, int pos, int head, int vector_bytes) {
+    return paged_vector_at(page, p.page_bytes, paged_slot_of(pos, p.page_shift), p.NKV, head, vector_bytes);
+}
+__device__ __forceinline__ long long paged_scale(const Paged& p, int page, int pos, int head) {
+    return paged_scale_at(page, p.scale_stride, paged_slot_of(pos, p.page_shift), p.NKV, head);
+}
 
 // ---- formats ----
 template <int FMT>

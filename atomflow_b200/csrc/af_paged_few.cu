@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const Paged p, c
     auto issue = [&](int j, int page) {
         if (j < n) {
             const int pos = (t0 + warp + kWarps * j) * KT + lane;
-            const long long mine = page < 0 ? -1 : page * p.page_bytes + ((long long)paged_slot(p, pos) * p.NKV + kvh) * F::kRow;
+            const long long mine = page < 0 ? -1 : paged_at(p, page, pos, kvh, F::kRow);
             const uint32_t stage = ring + (j % F::kStages) * (2 * F::kHalf);
             constexpr int RPI = 32 / F::kCh;   // rows of one warp-wide copy
             const int ch = lane % F::kCh;
@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(const Paged p, c
         if constexpr (FMT != AF_KV_F16) {
             if (page >= 0) {
                 const int pos = (t0 + warp + kWarps * j) * KT + lane;
-                const long long at = page * p.scale_stride + (long long)paged_slot(p, pos) * p.NKV + kvh;
+                const long long at = paged_scale(p, page, pos, kvh);
                 s = __halves2half2(__ldg(p.ks + at), __ldg(p.vs + at));
             }
         }

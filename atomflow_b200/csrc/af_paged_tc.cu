@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
                     for (int k = 0; k < KR; ++k) {
                         const int pos = j0 + r0 + k * RS;
                         const bool ok = pg[k] >= 0;
-                        const uint8_t* src = base + (ok ? pg[k] * p.page_bytes + ((long long)paged_slot(p, pos) * p.NKV + kvh) * (HD * 2) + c * 16 : 0);
+                        const uint8_t* src = base + (ok ? paged_at(p, pg[k], pos, kvh, HD * 2) + c * 16 : 0);
                         cp_async16_zfill(dst + k * RS * 128, src, ok ? 16u : 0u);
                     }
                 }
@@ -363,9 +363,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
                     code[k] = make_uint4(0u, 0u, 0u, 0u);
                     sc[k] = __float2half_rn(0.f);
                     if (page >= 0) {
-                        const long long slot = (long long)paged_slot(p, pos) * p.NKV + kvh;
-                        code[k] = __ldg(reinterpret_cast<const uint4*>(base + page * p.page_bytes + slot * HD + c * 16));
-                        sc[k] = __ldg(sbase + page * p.scale_stride + slot);
+                        code[k] = __ldg(reinterpret_cast<const uint4*>(base + paged_at(p, page, pos, kvh, HD) + c * 16));
+                        sc[k] = __ldg(sbase + paged_scale(p, page, pos, kvh));
                     }
                 }
             };
