@@ -9,11 +9,15 @@
 //   * Rows: the G query heads that share a kv head see the same K and V, so the
 //     rows of a work item are (token, head of the group) pairs of one sequence,
 //     256 of them: two 128-row MMA tiles that share every K and V tile read.
-//   * Warps 12-15 load: K and V tiles of 128 positions, row by row through the
-//     block table (16-byte cp.async for FP16; 8-bit codes pass through registers
-//     and are multiplied by their scale into FP16, the values af_paged_kv_read
-//     returns), into a ring of slots in the 128-byte-swizzled layout that the
-//     MMA reads.  Positions at or past the sequence's end are zeros.
+//   * Warp 9 fetches K and V tiles of 128 positions with TMA, one box per page (and
+//     64-dim panel) through the block table, into a ring of slots in the
+//     128-byte-swizzled layout that the MMA reads; a page outside the pool is a
+//     coordinate outside the tensor, which reads as zeros.  8-bit codes land in a
+//     staging ring, and warps 12-15 multiply them by their scales into FP16 slots
+//     (the values af_paged_kv_read returns).
+//   * V rows past the sequence's end would meet weights of zero, but what lies there
+//     may be NaN: warps 12-15 put zeros in their place.  (K rows there give scores
+//     that are masked.)
 //   * Warp 8 issues the MMAs.  S of both row tiles and O of both fill the 512
 //     TMEM columns; P (FP16) overwrites the S it came from and is the A operand
 //     of the second product straight from TMEM.  The order PV(0, j), QK(0, j+1),
@@ -31,6 +35,8 @@
 //   * Every wait is bounded; one that runs out sets AF_FAULT_TC_WAIT and the
 //     kernel ends without waiting further.
 #include <cooperative_groups.h>
+#include <cuda.h>
+#include <cudaTypedefs.h>
 
 #include <algorithm>
 #include <atomic>
@@ -44,20 +50,27 @@ namespace {
 constexpr int kTile = 128;              // rows of an MMA tile; positions of a K or V tile
 constexpr int kItemRows = 2 * kTile;
 constexpr int kThreads = 512;
-constexpr int kLoadWarp = 12, kMmaWarp = 8;
+constexpr int kMmaWarp = 8, kFetchWarp = 9, kConvWarp = 12;
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr int kMaxSplit = 8;
 constexpr float kGrow = 8.f;            // log2 of the growth of the maximum that forces a rescale
 constexpr int kTmemCols = 512;
 
-template <int HD>
+template <int FMT, int HD>
 struct Shape {
+    static constexpr bool kQuant = FMT != AF_KV_F16;
     static constexpr int kTileBytes = kTile * HD * 2;    // one 128 x HD FP16 tile
-    static constexpr int kSlots = HD == 128 ? 5 : 8;
+    static constexpr int kCodeBytes = kTile * HD;        // one 128 x HD tile of codes
+    static constexpr int kSlots = HD == 64 ? 8 : kQuant ? 4 : 5;
+    static constexpr int kStages = kQuant ? (HD == 64 ? 4 : 2) : 0;
     static constexpr int kQBytes = 2 * kTileBytes;
-    static constexpr size_t kSmem = kQBytes + (size_t)kSlots * kTileBytes + 1024;   // + alignment to 1 KB
+    static constexpr int kRing = kQBytes, kStaging = kRing + kSlots * kTileBytes;
+    static constexpr size_t kSmem = kStaging + (size_t)kStages * kCodeBytes + 1024;   // + alignment to 1 KB
+    // the fetch ring: slots, or staging for codes
+    static constexpr int kFetch = kQuant ? kStages : kSlots;
 };
-static_assert(Shape<128>::kSmem + 512 <= 227 * 1024, "shared memory");
+static_assert(Shape<AF_KV_F16, 128>::kSmem + 2048 <= 227 * 1024 && Shape<AF_KV_INT8, 128>::kSmem + 2048 <= 227 * 1024,
+              "shared memory");
 
 struct TcArgs {
     const __half* q;
@@ -149,6 +162,14 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint3
 __device__ __forceinline__ constexpr uint32_t instr_desc(int n, bool b_n_major) {
     return (1u << 4) | (b_n_major ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
 }
+// One box of a 5-D tensor -> shared memory, completing on an mbarrier.
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int c1, int c2, int c3, int c4, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], "
+        "[%7];" ::"r"(dst),
+        "l"(map), "r"(0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(bar)
+        : "memory");
+}
 __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, uint32_t n) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
@@ -179,10 +200,19 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     return r;
 }
 
+// One lane of a converged warp, in the form from which the compiler knows that a single thread follows (the MMA's
+// operands then stay in uniform registers).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(r));
+    return r != 0;
+}
+
 struct Bars {
-    uint64_t full[8], empty[8];    // ring slots
-    uint64_t s_full[2], p_full[2]; // per row tile
-    uint64_t o_done;
+    uint64_t full[8], empty[8];          // ring slots
+    uint64_t raw_full[4], raw_empty[4];  // staging of codes; FP16: the V tiles with masked positions (three at most)
+    uint64_t s_full[2], p_full[2];       // per row tile
+    uint64_t q_full, o_done;
 };
 
 // Bounded wait: false once the limit has passed (the fault bit is set).
@@ -197,14 +227,18 @@ __device__ __forceinline__ bool tc_wait(const uint64_t* bar, uint32_t parity, vo
 }
 
 template <int FMT, int HD>
-__global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p, const TcArgs a, unsigned* fault) {
+__global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p, const TcArgs a,
+                                                                   const __grid_constant__ CUtensorMap k_map,
+                                                                   const __grid_constant__ CUtensorMap v_map,
+                                                                   unsigned* fault) {
     namespace cg = cooperative_groups;
-    using Sh = Shape<HD>;
+    using Sh = Shape<FMT, HD>;
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) Bars bars;
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_abort;
     __shared__ int s_item[2];                        // sequence, row tile pair
+    __shared__ __half s_scale[2][2][kTile];          // two tiles' scales: K's, V's
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     cg::cluster_group cluster = cg::this_cluster();
@@ -250,9 +284,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
     }
     if (threadIdx.x == 32) {
         for (int i = 0; i < 8; ++i) {
-            mbar_init(smem_u32(&bars.full[i]), 128);
+            mbar_init(smem_u32(&bars.full[i]), Sh::kQuant ? 128 : 1);
             mbar_init(smem_u32(&bars.empty[i]), 1);
         }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(smem_u32(&bars.raw_full[i]), 1);
+            mbar_init(smem_u32(&bars.raw_empty[i]), 128);
+        }
+        mbar_init(smem_u32(&bars.q_full), 128);
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&bars.s_full[i]), 1);
             mbar_init(smem_u32(&bars.p_full[i]), 128);
@@ -279,23 +318,27 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
     const int tiles = (end + kTile - 1) / kTile;
     const int t0 = (int)((long long)tiles * rank / S), t1 = (int)((long long)tiles * (rank + 1) / S);
     const int n = t1 - t0;
+    // tiles from first_masked on hold positions that some row does not see
+    const int first_masked = max(0, max(0, ctx + row_base / a.G + 1) / kTile - t0);
     unsigned char* q_s = smem;
-    unsigned char* ring = smem + Sh::kQBytes;
+    unsigned char* ring = smem + Sh::kRing;
     // the cluster merge's parts, in the buffers once they are idle: FP32 O [256][HD], then m and l [256]
     float* part_o = reinterpret_cast<float*>(smem);
     float* part_m = part_o + kItemRows * HD;
     float* part_l = part_m + kItemRows;
     static_assert((kItemRows * HD + 2 * kItemRows) * 4 <= Sh::kSmem - 1024, "parts fit");
 
-    if (warp >= kLoadWarp) {
-        // ------------------------------------------------------------- loaders
-        // registers are handed over once, here, and never taken back: 2 x 184 + 48 + 96 = 4 x 128
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
-        const int i = threadIdx.x - kLoadWarp * 32;
-        constexpr int CH = HD / 8;                   // 16-byte FP16 chunks of a row
+    auto any_abort = [&] { return __any_sync(0xffffffffu, s_abort != 0) != 0; };   // the same for the whole warp
+
+    if (warp >= kConvWarp) {
+        // ------------------------------------------------ Q, conversion, mending
+        // registers are handed over once, here, and never taken back: 2 x 184 + 56 + 88 = 4 x 128
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        const int i = threadIdx.x - kConvWarp * 32;
         if (n > 0) {
-            const int c = i % CH, r0 = i / CH;
+            constexpr int CH = HD / 8;               // 16-byte FP16 chunks of a row
             constexpr int RS = 128 / CH;             // rows between a thread's rows (a multiple of 8)
+            const int c = i % CH, r0 = i / CH;
             const uint32_t at = smem_u32(q_s) + (c >> 3) * (kTile * 128) + r0 * 128 + (((c & 7) ^ (r0 & 7)) << 4);
 #pragma unroll 4
             for (int k = 0; k < kItemRows / RS; ++k) {
@@ -307,95 +350,85 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
                 cp_async16_zfill(at + (rt >> 7) * Sh::kTileBytes + (rt & 127) * 128, src, ok ? 16u : 0u);
             }
             cp_async_commit();
-        }
-        if constexpr (FMT == AF_KV_F16) {
-            constexpr int RS = 128 / CH, KR = kTile / RS;   // rows of a tile per thread
-            const int c = i % CH, r0 = i / CH;
-            const uint32_t at = (c >> 3) * (kTile * 128) + r0 * 128 + (((c & 7) ^ (r0 & 7)) << 4);
-            constexpr int D = 2;                            // tiles left in flight behind the newest
-            int pg[KR];
-            for (int m = 0; m < 2 * n + D; ++m) {
-                if (m < 2 * n) {
-                    const int slot = m % Sh::kSlots, j0 = (t0 + (m >> 1)) * kTile;
-                    if (!(m & 1)) {                         // K: look the pages up; V: the same
+            if constexpr (!Sh::kQuant) {
+                cp_async_wait<0>();
+                fence_async_smem();
+                mbar_arrive(smem_u32(&bars.q_full));
+                // V tiles with masked positions come by way of these warps: zeros past the end
+                for (int j = first_masked; j < n; ++j) {
+                    const int slot = (2 * j + 1) % Sh::kSlots;
+                    tc_wait(&bars.raw_full[j - first_masked], 0, &s_abort, fault);
+                    const int first = max(0, end - (t0 + j) * kTile);
+                    unsigned char* v = ring + slot * Sh::kTileBytes;
+                    for (int x = first * CH + i; x < kTile * CH; x += 128)   // zeros: the swizzle does not matter
+                        *reinterpret_cast<uint4*>(v + ((x % CH) >> 3) * (kTile * 128) + (x / CH) * 128 + (x & 7) * 16) =
+                            make_uint4(0u, 0u, 0u, 0u);
+                    fence_async_smem();
+                    named_bar_sync(1, 128);
+                    if (i == 0) mbar_arrive(smem_u32(&bars.full[slot]));
+                }
+            } else {
+                constexpr int C8 = HD / 16;          // 16-code chunks of a row
+                constexpr int RC = 128 / C8, KR = kTile / RC;
+                const int c8 = i % C8, q0 = i / C8;
+                // code chunk c8 makes FP16 chunks 2 c8 and 2 c8 + 1 of panel c8 / 4
+                const uint32_t row_at = (c8 >> 2) * (kTile * 128) + q0 * 128;
+                const uint32_t x0 = ((2 * c8) & 7) ^ (q0 & 7), x1 = ((2 * c8 + 1) & 7) ^ (q0 & 7);
+                __half sk, sv;                       // of position i of the next tile
+                auto fetch = [&](int j) {
+                    const int pos = (t0 + j) * kTile + i;
+                    sk = sv = __float2half_rn(0.f);
+                    const int page = j < n && pos < end ? paged_page(p, b, pos, fault) : -1;
+                    if (page >= 0) {
+                        const long long at = paged_scale(p, page, pos, kvh);
+                        sk = __ldg(p.ks + at);
+                        sv = __ldg(p.vs + at);
+                    }
+                };
+                fetch(0);
+                cp_async_wait<0>();
+                fence_async_smem();
+                mbar_arrive(smem_u32(&bars.q_full));
+                for (int j = 0; j < n; ++j) {
+                    s_scale[j & 1][0][i] = sk;
+                    s_scale[j & 1][1][i] = sv;
+                    named_bar_sync(1, 128);
+                    fetch(j + 1);
+                    const int left = end - (t0 + j) * kTile;   // positions of the tile that exist
+#pragma unroll
+                    for (int kv = 0; kv < 2; ++kv) {
+                        const int m = 2 * j + kv, slot = m % Sh::kSlots, st = m % Sh::kStages;
+                        tc_wait(&bars.raw_full[st], (m / Sh::kStages) & 1, &s_abort, fault);
+                        if (m >= Sh::kSlots) tc_wait(&bars.empty[slot], (m / Sh::kSlots - 1) & 1, &s_abort, fault);
+                        const unsigned char* src = smem + Sh::kStaging + st * Sh::kCodeBytes + i * 16;
+                        unsigned char* dst = ring + slot * Sh::kTileBytes + row_at;
 #pragma unroll
                         for (int k = 0; k < KR; ++k) {
-                            const int pos = j0 + r0 + k * RS;
-                            pg[k] = pos < end ? paged_page(p, b, pos, fault) : -1;
+                            const int r = q0 + k * RC;
+                            uint4 code = *reinterpret_cast<const uint4*>(src + k * 2048);
+                            if (r >= left) code = make_uint4(0u, 0u, 0u, 0u);
+                            const __half2 s2 = __half2half2(s_scale[j & 1][kv][r]);
+                            const uint32_t in[4] = {code.x, code.y, code.z, code.w};
+                            uint32_t o[8];
+#pragma unroll
+                            for (int w = 0; w < 4; ++w) {
+                                kv_unpack4<FMT>(in[w], o[2 * w], o[2 * w + 1]);
+                                o[2 * w] = mul_half2(o[2 * w], s2);
+                                o[2 * w + 1] = mul_half2(o[2 * w + 1], s2);
+                            }
+                            *reinterpret_cast<uint4*>(dst + k * RC * 128 + x0 * 16) = make_uint4(o[0], o[1], o[2], o[3]);
+                            *reinterpret_cast<uint4*>(dst + k * RC * 128 + x1 * 16) = make_uint4(o[4], o[5], o[6], o[7]);
                         }
-                    }
-                    if (m >= Sh::kSlots) tc_wait(&bars.empty[slot], (m / Sh::kSlots - 1) & 1, &s_abort, fault);
-                    const uint8_t* base = (m & 1) ? p.v : p.k;
-                    const uint32_t dst = smem_u32(ring) + slot * Sh::kTileBytes + at;
-#pragma unroll
-                    for (int k = 0; k < KR; ++k) {
-                        const int pos = j0 + r0 + k * RS;
-                        const bool ok = pg[k] >= 0;
-                        const uint8_t* src = base + (ok ? paged_at(p, pg[k], pos, kvh, HD * 2) + c * 16 : 0);
-                        cp_async16_zfill(dst + k * RS * 128, src, ok ? 16u : 0u);
+                        fence_async_smem();
+                        mbar_arrive(smem_u32(&bars.full[slot]));
+                        mbar_arrive(smem_u32(&bars.raw_empty[st]));
                     }
                 }
-                cp_async_commit();
-                if (m >= D) {
-                    cp_async_wait<D>();
-                    fence_async_smem();
-                    mbar_arrive(smem_u32(&bars.full[(m - D) % Sh::kSlots]));
-                }
-            }
-            cp_async_wait<0>();
-        } else {   // 8-bit
-            constexpr int C8 = HD / 16;                     // 16-code chunks of a row
-            constexpr int RS = 128 / C8, KR = kTile / RS;
-            const int c = i % C8, r0 = i / C8;
-            // code chunk c makes FP16 chunks 2c and 2c + 1 of panel c / 4
-            const uint32_t row_at = (c >> 2) * (kTile * 128) + r0 * 128;
-            const uint32_t x0 = ((2 * c) & 7) ^ (r0 & 7), x1 = ((2 * c + 1) & 7) ^ (r0 & 7);
-            uint4 code[KR];
-            __half sc[KR];
-            auto fetch = [&](int m) {
-                const int j0 = (t0 + (m >> 1)) * kTile;
-                const uint8_t* base = (m & 1) ? p.v : p.k;
-                const __half* sbase = (m & 1) ? p.vs : p.ks;
-#pragma unroll
-                for (int k = 0; k < KR; ++k) {
-                    const int pos = j0 + r0 + k * RS;
-                    const int page = pos < end ? paged_page(p, b, pos, fault) : -1;
-                    code[k] = make_uint4(0u, 0u, 0u, 0u);
-                    sc[k] = __float2half_rn(0.f);
-                    if (page >= 0) {
-                        code[k] = __ldg(reinterpret_cast<const uint4*>(base + paged_at(p, page, pos, kvh, HD) + c * 16));
-                        sc[k] = __ldg(sbase + paged_scale(p, page, pos, kvh));
-                    }
-                }
-            };
-            if (n > 0) fetch(0);
-            cp_async_wait<0>();                             // Q
-            for (int m = 0; m < 2 * n; ++m) {
-                const int slot = m % Sh::kSlots;
-                if (m >= Sh::kSlots) tc_wait(&bars.empty[slot], (m / Sh::kSlots - 1) & 1, &s_abort, fault);
-                unsigned char* dst = ring + slot * Sh::kTileBytes + row_at;
-#pragma unroll
-                for (int k = 0; k < KR; ++k) {
-                    const __half2 s2 = __half2half2(sc[k]);
-                    const uint32_t in[4] = {code[k].x, code[k].y, code[k].z, code[k].w};
-                    uint32_t o[8];
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        kv_unpack4<FMT>(in[w], o[2 * w], o[2 * w + 1]);
-                        o[2 * w] = mul_half2(o[2 * w], s2);
-                        o[2 * w + 1] = mul_half2(o[2 * w + 1], s2);
-                    }
-                    *reinterpret_cast<uint4*>(dst + k * RS * 128 + x0 * 16) = make_uint4(o[0], o[1], o[2], o[3]);
-                    *reinterpret_cast<uint4*>(dst + k * RS * 128 + x1 * 16) = make_uint4(o[4], o[5], o[6], o[7]);
-                }
-                fence_async_smem();
-                mbar_arrive(smem_u32(&bars.full[slot]));
-                if (m + 1 < 2 * n) fetch(m + 1);
             }
         }
     } else if (warp >= kMmaWarp) {
         // ----------------------------------------------------------- MMA issue
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == kMmaWarp) {
             constexpr uint32_t qk_desc = instr_desc(kTile, false), pv_desc = instr_desc(HD, true);
             const uint32_t q0 = smem_u32(q_s), r0 = smem_u32(ring);
@@ -421,8 +454,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
                 tc_fence_after();
             };
             if (n > 0) {
+                tc_wait(&bars.q_full, 0, &s_abort, fault);
                 full(0);
-                if (lane == 0 && !s_abort) {
+                if (!any_abort() && elect_one()) {
                     for (int i = 0; i < n_sub; ++i) qk(i, 0);
                     tc_commit(smem_u32(&bars.empty[0]));
                 }
@@ -433,21 +467,57 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
                     for (int i = 0; i < n_sub; ++i) {
                         tc_wait(&bars.p_full[i], j & 1, &s_abort, fault);
                         tc_fence_after();
-                        if (lane == 0 && !s_abort) pv(i, mv, j > 0);
+                        if (!any_abort() && elect_one()) pv(i, mv, j > 0);
                         __syncwarp();
                         if (j + 1 < n) {
                             if (i == 0) full(mk);
-                            if (lane == 0 && !s_abort) qk(i, mk);
+                            if (!any_abort() && elect_one()) qk(i, mk);
                             __syncwarp();
                         }
                     }
-                    if (lane == 0 && !s_abort) {
+                    if (!any_abort() && elect_one()) {
                         tc_commit(smem_u32(&bars.empty[mv % Sh::kSlots]));
                         if (j + 1 < n) tc_commit(smem_u32(&bars.empty[mk % Sh::kSlots]));
                         else tc_commit(smem_u32(&bars.o_done));
                     }
                     __syncwarp();
                 }
+            }
+        } else if (warp == kFetchWarp) {
+            // -------------------------------------------------------------- fetch
+            // one box per page of the tile and, for FP16, 64-dim panel: a lane each
+            constexpr int PN = Sh::kQuant ? 1 : HD / 64;
+            constexpr int kRow = Sh::kQuant ? HD : 128;      // bytes of a box's row
+            const int box_rows = min(1 << p.page_shift, kTile);
+            const int panel = lane % PN, box = lane / PN;
+            uint64_t* fetched = Sh::kQuant ? bars.raw_full : bars.full;
+            uint64_t* empty = Sh::kQuant ? bars.raw_empty : bars.empty;
+            const uint32_t base = smem_u32(smem + (Sh::kQuant ? Sh::kStaging : Sh::kRing)) + panel * (kTile * 128) +
+                                  box * box_rows * kRow;
+            int page = 0, m = 0;
+            for (; m < 2 * n && !any_abort(); ++m) {
+                const int st = m % Sh::kFetch, pos0 = (t0 + (m >> 1)) * kTile;
+                const int boxes = (min(kTile, end - pos0) + box_rows - 1) / box_rows;   // those with positions that exist
+                const int pos = pos0 + box * box_rows;
+                if (!(m & 1) && box < boxes) {               // K: look the page up; V: the same
+                    page = paged_page(p, b, pos, fault);
+                    if (page < 0) page = max(p.n_pages, 1);  // outside the tensor: zeros
+                }
+                if (m >= Sh::kFetch) tc_wait(&empty[st], (m / Sh::kFetch - 1) & 1, &s_abort, fault);
+                // a V tile with masked positions: warps 12-15 hand it on
+                const int mask = (m & 1) && !Sh::kQuant ? (m >> 1) - first_masked : -1;
+                const uint32_t bar = smem_u32(mask >= 0 ? &bars.raw_full[mask] : &fetched[st]);
+                if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(boxes * box_rows * kRow * PN));
+                __syncwarp();
+                if (box < boxes)
+                    tma_load(base + st * (Sh::kQuant ? Sh::kCodeBytes : Sh::kTileBytes), (m & 1) ? &v_map : &k_map,
+                             paged_slot_of(pos, p.page_shift), panel, kvh, page, bar);
+            }
+            if (any_abort()) {   // nothing may still be landing when the CTA ends
+                for (int x = max(0, m - Sh::kFetch); x < m; ++x)
+                    mbar_wait_bounded(smem_u32(&fetched[x % Sh::kFetch]), (x / Sh::kFetch) & 1, kWaitNs);
+                for (int x = 0; !Sh::kQuant && x < n - first_masked; ++x)
+                    if (2 * (first_masked + x) + 1 < m) mbar_wait_bounded(smem_u32(&bars.raw_full[x]), 0, kWaitNs);
             }
         }
     } else {
@@ -616,22 +686,67 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
     }
 }
 
+// cuTensorMapEncodeTiled, taken from the driver at run time (the library does not link against it).
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encode(cudaError_t* err) {
+    static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> fn{nullptr};
+    auto f = fn.load(std::memory_order_acquire);
+    *err = cudaSuccess;
+    if (f == nullptr) {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult res = cudaDriverEntryPointSymbolNotFound;
+        *err = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &ptr, 12000, cudaEnableDefault, &res);
+        if (*err == cudaSuccess && (res != cudaDriverEntryPointSuccess || ptr == nullptr)) *err = cudaErrorNotSupported;
+        if (*err != cudaSuccess) return nullptr;
+        f = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+        fn.store(f, std::memory_order_release);
+    }
+    return f;
+}
+
+// The pool's K or V as a tensor [page][kv head][panel][slot][row bytes]: a box is one page's (at most 128) slots of one
+// head and one 128-byte panel (FP16) or whole vector (codes).
+template <int FMT, int HD>
+cudaError_t pool_map(CUtensorMap* map, const uint8_t* base, const Paged& p) {
+    cudaError_t e;
+    auto encode = tensor_map_encode(&e);
+    if (encode == nullptr) return e;
+    constexpr bool quant = FMT != AF_KV_F16;
+    constexpr int esz = KvFormat<FMT>::kBytes, inner = quant ? HD : 64, panels = HD / inner;
+    const cuuint64_t row = (cuuint64_t)p.NKV * HD * esz;
+    const int page = 1 << p.page_shift;
+    const cuuint64_t dims[5] = {(cuuint64_t)inner, (cuuint64_t)page, (cuuint64_t)panels, (cuuint64_t)p.NKV,
+                                (cuuint64_t)std::max(1, p.n_pages)};
+    const cuuint64_t strides[4] = {row, (cuuint64_t)inner * esz, (cuuint64_t)HD * esz, (cuuint64_t)p.page_bytes};
+    const cuuint32_t box[5] = {(cuuint32_t)inner, (cuuint32_t)std::min(page, kTile), 1, 1, 1};
+    const cuuint32_t step[5] = {1, 1, 1, 1, 1};
+    const CUresult r = encode(map, quant ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
+                              const_cast<uint8_t*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              quant ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 template <int FMT, int HD>
 cudaError_t launch(const Paged& p, const TcArgs& a, unsigned clusters, int S, unsigned* fault, cudaStream_t st) {
     auto kernel = paged_chunk_kernel<FMT, HD>;
+    using Sh = Shape<FMT, HD>;
     static std::atomic<bool> set[kMaxDevices];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev >= kMaxDevices || !set[dev].load(std::memory_order_acquire)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<HD>::kSmem);
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::kSmem);
         if (e != cudaSuccess) return e;
         if (dev < kMaxDevices) set[dev].store(true, std::memory_order_release);
     }
+    CUtensorMap k_map, v_map;
+    e = pool_map<FMT, HD>(&k_map, p.k, p);
+    if (e == cudaSuccess) e = pool_map<FMT, HD>(&v_map, p.v, p);
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(clusters * S);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = Shape<HD>::kSmem;
+    cfg.dynamicSmemBytes = Sh::kSmem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -639,7 +754,7 @@ cudaError_t launch(const Paged& p, const TcArgs& a, unsigned clusters, int S, un
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, p, a, fault);
+    return cudaLaunchKernelEx(&cfg, kernel, p, a, k_map, v_map, fault);
 }
 
 }  // namespace
