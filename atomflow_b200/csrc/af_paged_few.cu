@@ -161,25 +161,41 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
         }
         return x;
     };
-    // Copies tile j into its stage: lane l takes chunk l % kCh of every (32 / kCh)-th row.
-    const int ch = lane % F::kCh, row_of = lane / F::kCh;
-    const long long row_bytes = (long long)p.NKV * F::kRow;
-    const long long lane_off = (long long)row_of * row_bytes + ch * 16;
+    // Copies tile j into its stage: lane l takes chunk l % kCh of every (32 / kCh)-th row.  The rows of one lane are
+    // RPI apart, so their places in the stage differ by constants.
+    constexpr int RPI = 32 / F::kCh;                 // rows of one warp-wide copy, at most 8
+    constexpr int half = 8 / RPI;                    // copies per half tile
+    const int row_of = lane / F::kCh;
+    const long long row_bytes = (long long)p.NKV * F::kRow, step = RPI * row_bytes;
+    const long long lane_off = (long long)row_of * row_bytes + (lane % F::kCh) * 16 + (long long)kvh * F::kRow;
+    const uint8_t *k_lane = p.k + lane_off, *v_lane = p.v + lane_off;
+    uint32_t k_to[KT / RPI], v_to[KT / RPI];
+#pragma unroll
+    for (int i = 0; i < KT / RPI; ++i) {
+        k_to[i] = F::at(row_of + i * RPI, lane % F::kCh, false);
+        v_to[i] = F::kHalf + F::at(row_of + i * RPI, lane % F::kCh, true);
+    }
     auto issue = [&](int j, Pages pg) {
         if (j < n) {
             const int pos = (t0 + warp + W * j) * KT;
             const uint32_t stage = ring + (j % F::kStages) * (2 * F::kHalf);
-            constexpr int RPI = 32 / F::kCh;         // rows of one warp-wide copy, at most 8
-            const long long lo = paged_at(p, max(pg.lo, 0), pos, kvh, F::kRow) + lane_off;
-            const long long hi = paged_at(p, max(pg.hi, 0), pos + 8, kvh, F::kRow) + lane_off;
+            const long long lo = paged_at(p, max(pg.lo, 0), pos, 0, F::kRow);
+            const long long hi = p.page_shift > 3 ? lo + 8 * row_bytes : paged_at(p, max(pg.hi, 0), pos, 0, F::kRow);
+            if ((pg.lo | pg.hi) >= 0 && pos + KT <= end) {
 #pragma unroll
-            for (int i = 0; i < KT / RPI; ++i) {
-                const int r = row_of + i * RPI;
-                constexpr int half = 8 / RPI;        // copies per half
-                const bool ok = (i < half ? pg.lo : pg.hi) >= 0 && pos + r < end;
-                const long long src = ok ? (i < half ? lo : hi) + (i % half) * RPI * row_bytes : 0;
-                cp_async16_zfill(stage + F::at(r, ch, false), p.k + src, ok ? 16u : 0u);
-                cp_async16_zfill(stage + F::kHalf + F::at(r, ch, true), p.v + src, ok ? 16u : 0u);
+                for (int i = 0; i < KT / RPI; ++i) {
+                    const long long src = (i < half ? lo : hi) + (i % half) * step;
+                    cp_async16(stage + k_to[i], k_lane + src);
+                    cp_async16(stage + v_to[i], v_lane + src);
+                }
+            } else {   // positions past the end, or without a page: zeros
+#pragma unroll
+                for (int i = 0; i < KT / RPI; ++i) {
+                    const bool ok = (i < half ? pg.lo : pg.hi) >= 0 && pos + row_of + i * RPI < end;
+                    const long long src = ok ? (i < half ? lo : hi) + (i % half) * step : 0;
+                    cp_async16_zfill(stage + k_to[i], ok ? k_lane + src : p.k, ok ? 16u : 0u);
+                    cp_async16_zfill(stage + v_to[i], ok ? v_lane + src : p.v, ok ? 16u : 0u);
+                }
             }
         }
         cp_async_commit();
@@ -246,6 +262,10 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
         }
     }
     const int seen_by_all = max(0, ctx + 1);         // positions that no row masks
+    // Places of the lane's operands in a stage: for 8-bit, the chunks of one row differ by an xor, rows by constants
+    // (F::at's permutation of rows 2c, 2c + 1, 2c + 8, 2c + 9, and of g, g + 8, is one).
+    const uint32_t k_at = FMT == AF_KV_F16 ? 0u : F::at(g, c, false);
+    const uint32_t v_at = FMT == AF_KV_F16 ? 0u : F::at(2 * c, g >> 2, true) + (uint32_t)((g & 3) * 4);
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -284,8 +304,8 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
         } else {
 #pragma unroll
             for (int u = 0; u < HD / 64; ++u) {
-                const uint4 x = lds128(ks + F::at(g, 4 * u + c, false));
-                const uint4 y = lds128(ks + F::at(g + 8, 4 * u + c, false));
+                const uint4 x = lds128(ks + (k_at ^ (u * 64)));
+                const uint4 y = lds128(ks + (k_at ^ (u * 64)) + 8 * F::kRow);
                 const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
@@ -383,10 +403,10 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
             const __half2 s89 = __halves2half2(__shfl_sync(0xffffffffu, sc, 24 + k), __shfl_sync(0xffffffffu, sc, 25 + k));
 #pragma unroll
             for (int d = 0; d < HD / 32; ++d) {   // the lane's dims: 32 d + 4 g + 0..3
-                const int vc = 2 * d + (g >> 2);
-                const uint32_t in = (uint32_t)((g & 3) * 4);
-                const uint32_t w0 = lds32(vs + F::at(k, vc, true) + in), w1 = lds32(vs + F::at(k + 1, vc, true) + in);
-                const uint32_t w8 = lds32(vs + F::at(k + 8, vc, true) + in), w9 = lds32(vs + F::at(k + 9, vc, true) + in);
+                const uint32_t at = vs + (v_at ^ (d * 32));
+                const uint32_t w0 = lds32(at), w1 = lds32((HD == 64 ? vs + (v_at ^ (d * 32) ^ 64) : at + F::kRow));
+                const uint32_t w8 = lds32(at + 8 * F::kRow);
+                const uint32_t w9 = lds32((HD == 64 ? vs + (v_at ^ (d * 32) ^ 64) : at + F::kRow) + 8 * F::kRow);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {   // dims 2h and 2h + 1 of the four
                     uint32_t a0, a1, a2, a3;
