@@ -128,7 +128,8 @@ C_SYMBOLS = {
     "af_gemv_chain_fast": (_i, [ctypes.c_void_p, _i, _vp, _sz, _vp]),
     "af_paged_kv_write": (_i, [_vp, _vp, _vp, _i64, _i, _vp, _vp, _i, _vp, _vp]),
     "af_paged_kv_read": (_i, [_vp, _vp, _vp, _vp, _vp]),
-    "af_paged_attention": (_i, [_vp, _vp, _vp, _i64, _i, ctypes.c_float, _i, _i, _vp, _vp]),
+    "af_paged_attention_workspace_bytes": (_sz, [_vp, _vp, _i, _i, _i]),
+    "af_paged_attention": (_i, [_vp, _vp, _vp, _i64, _i, ctypes.c_float, _i, _i, _vp, _vp, _sz, _vp]),
     "af_engine_create": (_i, [ctypes.c_char_p, _i, _i, _i, ctypes.POINTER(ctypes.c_void_p)]),
     "af_engine_create_tp": (_i, [ctypes.c_char_p, _i, _i, _vp, ctypes.POINTER(ctypes.c_void_p)]),
     "af_engine_destroy": (_i, [_vp]),

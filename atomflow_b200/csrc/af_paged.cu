@@ -351,35 +351,66 @@ extern "C" af_status af_paged_kv_read(const af_paged_kv* kv, const af_paged_batc
     return e == cudaSuccess ? AF_OK : cuda_fail(e, "paged_read_kernel");
 }
 
+namespace {
+
+// Which kernels an attention call runs.  Which sequences each takes is a matter of their rows (new tokens x query heads
+// per kv head), which only the device knows; the host's bounds say which kernels can have work.
+struct AttnPlan {
+    bool few, chunk;    // sequences of at most kFewRows rows; longer ones
+    int few_rows;       // bound on the rows of the former
+    int skip_rows;      // the chunk kernel leaves sequences of at most these to the other
+    int kv;             // bound on the cached positions
+};
+AttnPlan attn_plan(const Paged& p, int n_heads, int max_rows, int max_kv) {
+    AttnPlan x;
+    const long long cap = (long long)p.max_pages << p.page_shift;
+    x.kv = (int)std::min<long long>({max_kv > 0 ? (long long)max_kv : cap, cap, INT_MAX});
+    const int q = max_rows > 0 ? std::min(max_rows, p.n_tokens) : p.n_tokens;
+    const long long rows = (long long)q * (n_heads / p.NKV);
+    const bool even = (long long)q * p.n_seqs <= p.n_tokens;   // every sequence as long as the bound: none is short
+    x.chunk = rows > kFewRows;
+    x.few = !x.chunk || !even;
+    x.few_rows = (int)std::min<long long>(rows, kFewRows);
+    x.skip_rows = even ? 0 : kFewRows;
+    return x;
+}
+
+af_status attn_args(const af_paged_kv* kv, const af_paged_batch* batch, int n_heads, int max_rows, int max_kv, Paged* p) {
+    const af_status st = paged_args(kv, batch, p);
+    if (st != AF_OK) return st;
+    if (n_heads < 1 || n_heads > 65535 || n_heads % p->NKV != 0 || max_rows < 0 || max_kv < 0) return AF_ERR_INVALID;
+    return (long long)p->n_tokens * (n_heads / p->NKV) > INT_MAX ? AF_ERR_UNSUPPORTED : AF_OK;
+}
+
+}  // namespace
+
+extern "C" size_t af_paged_attention_workspace_bytes(const af_paged_kv* kv, const af_paged_batch* batch, int n_heads,
+                                                     int max_rows, int max_kv) {
+    Paged p;
+    if (attn_args(kv, batch, n_heads, max_rows, max_kv, &p) != AF_OK || p.n_seqs == 0 || p.n_tokens == 0) return 0;
+    const AttnPlan x = attn_plan(p, n_heads, max_rows, max_kv);
+    return x.few ? paged_few_workspace(kv->format, kv->head_dim, p, x.few_rows, x.kv) : 0;
+}
+
 extern "C" af_status af_paged_attention(const af_paged_kv* kv, const af_paged_batch* batch, const void* q,
                                         int64_t q_stride, int n_heads, float scale, int max_rows, int max_kv,
-                                        void* out, void* stream) {
+                                        void* out, void* workspace, size_t workspace_bytes, void* stream) {
     Paged p;
-    const af_status st = paged_args(kv, batch, &p);
+    const af_status st = attn_args(kv, batch, n_heads, max_rows, max_kv, &p);
     if (st != AF_OK) return st;
-    if (n_heads < 1 || n_heads > 65535 || n_heads % p.NKV != 0) return AF_ERR_INVALID;
     if (q_stride < (int64_t)n_heads * kv->head_dim || q_stride % 8 != 0) return AF_ERR_INVALID;
-    if (!(scale > 0.f) || !std::isfinite(scale) || max_rows < 0 || max_kv < 0) return AF_ERR_INVALID;
+    if (!(scale > 0.f) || !std::isfinite(scale) || !aligned(workspace, 16)) return AF_ERR_INVALID;
     if (p.n_seqs == 0 || p.n_tokens == 0) return AF_OK;
     if (q == nullptr || out == nullptr || !aligned(q, 16) || !aligned(out, 16)) return AF_ERR_INVALID;
     cudaError_t e;
     unsigned* fault = paged_fault_word(&e);
     if (fault == nullptr) return cuda_fail(e, "af_paged_attention");
-    const long long cap = (long long)p.max_pages << p.page_shift;
-    const int kv_bound = (int)std::min<long long>(max_kv > 0 ? max_kv : cap, cap);
-    // Which kernel takes which sequences is a matter of their rows (new tokens x query heads per kv head), which only
-    // the device knows; the host's bound says which kernels can have work.
+    const AttnPlan x = attn_plan(p, n_heads, max_rows, max_kv);
     const cudaStream_t cs = static_cast<cudaStream_t>(stream);
-    const int q_bound = max_rows > 0 ? std::min(max_rows, p.n_tokens) : p.n_tokens;
-    const long long rows_bound = (long long)q_bound * (n_heads / p.NKV);
-    const bool few = rows_bound <= kFewRows;
-    // every sequence as long as the bound: none is short
-    const bool even = (long long)q_bound * p.n_seqs <= p.n_tokens;
-    if (few || !even)
-        e = paged_few_launch(kv->format, kv->head_dim, p, q, q_stride, n_heads, scale, few ? (int)rows_bound : kFewRows,
-                             few, kv_bound, out, fault, cs);
-    if (!few && e == cudaSuccess)
-        e = paged_chunk_launch(kv->format, kv->head_dim, p, q, q_stride, n_heads, scale, even ? 0 : kFewRows, kv_bound,
-                               out, fault, cs);
+    if (x.few)
+        e = paged_few_launch(kv->format, kv->head_dim, p, q, q_stride, n_heads, scale, x.few_rows, !x.chunk, x.kv, out,
+                             workspace, workspace_bytes, fault, cs);
+    if (x.chunk && e == cudaSuccess)
+        e = paged_chunk_launch(kv->format, kv->head_dim, p, q, q_stride, n_heads, scale, x.skip_rows, x.kv, out, fault, cs);
     return e == cudaSuccess ? AF_OK : cuda_fail(e, "af_paged_attention");
 }

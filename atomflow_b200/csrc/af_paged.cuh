@@ -149,9 +149,10 @@ af_status paged_args(const af_paged_kv* kv, const af_paged_batch* batch, Paged* 
 // The attention of few rows (af_paged_few.cu): every sequence of at most 8 (rows_bound <= 8) or kFewRows rows (tokens x
 // query heads per kv head).  alone: sequences of more rows are recorded as a fault, no other kernel takes them.
 constexpr int kFewRows = 16;
+size_t paged_few_workspace(int format, int head_dim, const Paged& p, int rows_bound, int max_kv);
 cudaError_t paged_few_launch(int format, int head_dim, const Paged& p, const void* q, long long q_stride, int n_heads,
-                             float scale, int rows_bound, bool alone, int max_kv, void* out, unsigned* fault,
-                             cudaStream_t st);
+                             float scale, int rows_bound, bool alone, int max_kv, void* out, void* workspace,
+                             size_t workspace_bytes, unsigned* fault, cudaStream_t st);
 // The tensor-core attention (af_paged_tc.cu) over every sequence of more than
 // skip_rows rows (tokens x query heads per kv head).
 cudaError_t paged_chunk_launch(int format, int head_dim, const Paged& p, const void* q, long long q_stride, int n_heads,

@@ -2,10 +2,19 @@
 // drafted ones) over a paged KV cache: af_paged_attention's path for sequences
 // of at most 16 (token, query head) rows per kv head.
 //
-// Bound by reading the cache once.  A cluster of S CTAs takes one (sequence, kv
-// head); each CTA a contiguous share of its positions, each of its warps every
-// W-th tile of 16 positions, in a cp.async ring of its own (no CTA-wide barrier in
-// the loop).  Per tile, on m16n8k16 MMAs with the roles swapped so that 8 rows do
+// Bound by reading the cache once.  An item is one (sequence, kv head); its
+// positions go in tiles of 16, each of a CTA's W warps taking every W-th tile of
+// the CTA's range in a cp.async ring of its own (no CTA-wide barrier in the loop).
+// The work is divided over CTAs in one of two ways:
+//   * clusters (short caches): S CTAs share an item and merge through distributed
+//     shared memory -- one launch, no workspace;
+//   * one wave (long caches, with a workspace): all items' tiles in a row, cut
+//     into equal pieces, one per CTA that the GPU holds at once, so neither ragged
+//     lengths nor a single long sequence leaves SMs idle.  An item's pieces go to
+//     the workspace and a second, dependent launch merges them.  (One sequence of
+//     131,001 FP8 positions over 8 heads: clusters of 16, of which the GPU holds
+//     7, took 102 us.)
+// Per tile, on m16n8k16 MMAs with the roles swapped so that 8 rows do
 // not waste a 16-row operand:
 //   S^T [positions x rows] = K Q^T        K from shared memory, Q in registers
 //   O^T [dims x rows]     += V^T P^T      P^T turned round by movmatrix
@@ -21,8 +30,7 @@
 //   * K's scale multiplies S in FP32; V is scaled into FP16 (the values
 //     af_paged_kv_read returns), as P has no room for a scale that may be
 //     subnormal in FP16.  P is rounded to FP16.
-//   * Warps merge in shared memory, CTAs through distributed shared memory, in
-//     order: one launch, no workspace, the same bits every time.
+//   * Warps and CTAs merge in a fixed order: the same bits every time.
 //   * The loop is bound by issue slots as much as by DRAM: 8 warps per SM (two per
 //     scheduler) issued in 45% of the cycles and read the cache at 3.6 TB/s, so
 //     the rings are short and the registers few enough for 16 (12 with 16 rows
@@ -38,8 +46,10 @@
 namespace af {
 namespace {
 
-constexpr int kMaxSplit = 16;
+constexpr int kMaxSplit = 8;
+constexpr int kMergeThreads = 512;
 constexpr int KT = 16;             // positions of a tile
+constexpr int kLong = 512;         // positions per CTA of a cluster past which the work is cut into one wave
 constexpr float kGrow = 8.f;       // log2 of the growth of a score over the maximum that moves it
 
 // NT: 8-row column tiles; BIG: one CTA per SM with all its warps, else CTAs of four warps.
@@ -77,6 +87,9 @@ struct FewArgs {
     int NH, G;
     float c;       // scale * log2(e)
     int alone;     // no other kernel takes the sequences of too many rows: record them
+    float4* part_o;   // one wave: partial O [2 ctas][ROWS][HD], m and l [2 ctas][ROWS]
+    float2* part_ml;
+    int ctas;
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
@@ -123,7 +136,58 @@ __device__ __forceinline__ void unpack4_offset(uint32_t w, uint32_t& lo, uint32_
     hi = __byte_perm(w, 0x64646464u, 0x4342);
 }
 
-template <int FMT, int HD, int NT, bool BIG>
+// ---- one wave: every item's tiles in a row, sequence by sequence, head by head ----
+// Tiles of one head of sequence b; 0: not a sequence of ours.  (One without positions has an empty tile: its rows are
+// zeros that someone has to write.)
+template <int ROWS>
+__device__ __forceinline__ int few_tiles(const Paged& p, const FewArgs& a, int b, unsigned* fault) {
+    const PagedSeq s = paged_seq(p, b, fault);
+    const long long rows = (long long)s.q * a.G;
+    if (rows == 0 || rows > ROWS) {
+        if (rows > ROWS && a.alone) atomicOr(fault, (unsigned)AF_FAULT_PAGED);
+        return 0;
+    }
+    return max(1, (s.kv + KT - 1) / KT);
+}
+// By one whole warp: tiles of one head of sequences [0, n).
+template <int ROWS>
+__device__ long long few_sum(const Paged& p, const FewArgs& a, int n, unsigned* fault) {
+    long long t = 0;
+    for (int b = threadIdx.x & 31; b < n; b += 32) t += few_tiles<ROWS>(p, a, b, fault);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) t += __shfl_xor_sync(0xffffffffu, t, x);
+    return t;
+}
+// By one whole warp: the sequence that holds tile u of the row (u < all tiles), and its first tile.
+template <int ROWS>
+__device__ int few_find(const Paged& p, const FewArgs& a, long long u, long long& first, unsigned* fault) {
+    const int lane = threadIdx.x & 31;
+    long long seen = 0;
+    for (int b0 = 0; b0 < p.n_seqs; b0 += 32) {
+        const long long t = b0 + lane < p.n_seqs ? (long long)few_tiles<ROWS>(p, a, b0 + lane, fault) * p.NKV : 0;
+        long long inc = t;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, inc, x);
+            if (lane >= x) inc += y;
+        }
+        const unsigned who = __ballot_sync(0xffffffffu, u >= seen + inc - t && u < seen + inc);
+        if (who != 0) {
+            const int src = __ffs(who) - 1;
+            first = seen + __shfl_sync(0xffffffffu, inc - t, src);
+            return b0 + src;
+        }
+        seen += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    return -1;
+}
+// Tiles per CTA: an equal share, at least two per warp.
+__device__ __forceinline__ long long few_share(long long total, int ctas, int W) {
+    const long long u = (total + ctas - 1) / ctas;
+    return u < 2 * W ? 2 * W : u;
+}
+
+template <int FMT, int HD, int NT, bool BIG, bool WAVE>
 __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, NT, BIG>::kMinCtas)
     paged_few_kernel(const Paged p, const FewArgs a, unsigned* fault) {
     namespace cg = cooperative_groups;
@@ -132,19 +196,62 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ float s_m[W][ROWS], s_l[W][ROWS];
     __shared__ float c_m[ROWS], c_l[ROWS];   // this CTA's, for the cluster
-    cg::cluster_group cluster = cg::this_cluster();
-    const int S = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    const int cid = blockIdx.x / S, b = cid / p.NKV, kvh = cid - b * p.NKV;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const PagedSeq seq = paged_seq(p, b, fault);
-    const int rows = (int)min((long long)seq.q * a.G, (long long)ROWS + 1);
-    if (rows == 0 || rows > ROWS) {   // the whole cluster leaves
-        if (rows > ROWS && a.alone && threadIdx.x == 0) atomicOr(fault, (unsigned)AF_FAULT_PAGED);
-        return;
+    int S = 1, rank = 0, b, kvh, t0, t1;
+    PagedSeq seq;
+    long long u0 = 0, u1 = 0, first = 0;     // one wave: this CTA's tiles; first tile of sequence b
+    if constexpr (WAVE) {
+        pdl_launch_dependents();             // every CTA is resident: the merge may line up behind them
+        __shared__ long long s_first, s_u0, s_u1;
+        __shared__ int s_b;
+        if (warp == 0) {
+            const long long total = few_sum<ROWS>(p, a, p.n_seqs, fault) * p.NKV;
+            const long long share = few_share(total, a.ctas, W);
+            const long long lo = (long long)blockIdx.x * share, hi = min(total, lo + share);
+            long long f = 0;
+            const int at = lo < hi ? few_find<ROWS>(p, a, lo, f, fault) : -1;
+            if (lane == 0) {
+                s_u0 = lo;
+                s_u1 = hi;
+                s_first = f;
+                s_b = at;
+            }
+        }
+        __syncthreads();
+        b = s_b;
+        u0 = s_u0;
+        u1 = s_u1;
+        first = s_first;
+        if (b < 0) return;
+    } else {
+        cg::cluster_group cluster = cg::this_cluster();
+        S = (int)cluster.num_blocks();
+        rank = (int)cluster.block_rank();
+        const int cid = blockIdx.x / S;
+        b = cid / p.NKV;
+        kvh = cid - b * p.NKV;
+        seq = paged_seq(p, b, fault);
+        const long long rows = (long long)seq.q * a.G;
+        if (rows == 0 || rows > ROWS) {      // the whole cluster leaves
+            if (rows > ROWS && a.alone && threadIdx.x == 0) atomicOr(fault, (unsigned)AF_FAULT_PAGED);
+            return;
+        }
     }
+  for (;;) {   // one wave: every piece of an item that falls into this CTA's tiles
+    int tiles;
+    if constexpr (WAVE) {
+        seq = paged_seq(p, b, fault);
+        tiles = max(1, (seq.kv + KT - 1) / KT);
+        kvh = (int)((u0 - first) / tiles);
+        t0 = (int)(u0 - first - (long long)kvh * tiles);
+        t1 = (int)min((long long)tiles, t0 + (u1 - u0));
+    } else {
+        tiles = (seq.kv + KT - 1) / KT;
+        t0 = (int)((long long)tiles * rank / S);
+        t1 = (int)((long long)tiles * (rank + 1) / S);
+    }
+    const int rows = seq.q * a.G;
     const int ctx = seq.kv - seq.q, end = seq.kv;    // the last row sees every position
-    const int tiles = (end + KT - 1) / KT;
-    const int t0 = (int)((long long)tiles * rank / S), t1 = (int)((long long)tiles * (rank + 1) / S);
     const int n = (t1 - t0 - warp + W - 1) / W;      // this warp's tiles: t0 + warp + W * j
     const uint32_t ring = smem_u32(smem) + warp * (F::kStages * 2 * F::kHalf);
 
@@ -155,7 +262,7 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
     auto find = [&](int j) {
         Pages x{-1, -1};
         const int pos = (t0 + warp + W * j) * KT;
-        if (j < n) {
+        if (j < n && pos < end) {
             x.lo = paged_page(p, b, pos, fault);
             x.hi = p.page_shift > 3 ? x.lo : pos + 8 < end ? paged_page(p, b, pos + 8, fault) : -1;
         }
@@ -472,7 +579,11 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
             L = fmaf(s_l[w][r], f, L);
             add(v, reinterpret_cast<const float4*>(part)[(w * ROWS + r) * (HD / 4) + ch], f);
         }
-        if (S == 1) {
+        if (WAVE && t1 - t0 < tiles) {   // a piece of an item: the one that begins it, or a later one
+            const long long at = ((long long)2 * blockIdx.x + (t0 == 0 ? 1 : 0)) * ROWS + r;
+            a.part_o[at * (HD / 4) + ch] = v;
+            if (ch == 0) a.part_ml[at] = make_float2(M, L);
+        } else if (S == 1) {
             store(r, ch, v, L > 0.f ? 1.f / L : 0.f);
         } else {
             mine[r * (HD / 4) + ch] = v;
@@ -482,77 +593,210 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
             }
         }
     }
-    if (S > 1) {
-        cluster.sync();   // every CTA's part is there
-        const int total = rows * (HD / 4), lo = total * rank / S, hi = total * (rank + 1) / S;
-        for (int x = lo + threadIdx.x; x < hi; x += F::kThreads) {
-            const int r = x / (HD / 4), ch = x % (HD / 4);
-            float M = -INFINITY, L = 0.f;
-            for (int u = 0; u < S; ++u) M = fmaxf(M, cluster.map_shared_rank(c_m, u)[r]);
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-            for (int u = 0; u < S; ++u) {   // rank order: the same bits every time
-                const float mu = cluster.map_shared_rank(c_m, u)[r];
-                const float f = mu == -INFINITY ? 0.f : ex2(mu - M);
-                L = fmaf(cluster.map_shared_rank(c_l, u)[r], f, L);
-                add(v, cluster.map_shared_rank(mine, u)[r * (HD / 4) + ch], f);
-            }
-            store(r, ch, v, L > 0.f ? 1.f / L : 0.f);
+    if constexpr (WAVE) {
+        u0 += t1 - t0;
+        if (u0 >= u1) return;
+        if (u0 - first >= (long long)tiles * p.NKV) {   // on to the next sequence that is ours
+            first += (long long)tiles * p.NKV;
+            do ++b;
+            while (b < p.n_seqs && few_tiles<ROWS>(p, a, b, fault) == 0);
+            if (b >= p.n_seqs) return;
         }
-        cluster.sync();   // no CTA leaves while another reads its part
+        __syncthreads();   // the parts have been read: the rings are free
+    } else {
+        if (S > 1) {
+            cg::cluster_group cluster = cg::this_cluster();
+            cluster.sync();   // every CTA's part is there
+            const int total = rows * (HD / 4), lo = total * rank / S, hi = total * (rank + 1) / S;
+            for (int x = lo + threadIdx.x; x < hi; x += F::kThreads) {
+                const int r = x / (HD / 4), ch = x % (HD / 4);
+                float M = -INFINITY, L = 0.f;
+                for (int u = 0; u < S; ++u) M = fmaxf(M, cluster.map_shared_rank(c_m, u)[r]);
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+                for (int u = 0; u < S; ++u) {   // rank order: the same bits every time
+                    const float mu = cluster.map_shared_rank(c_m, u)[r];
+                    const float f = mu == -INFINITY ? 0.f : ex2(mu - M);
+                    L = fmaf(cluster.map_shared_rank(c_l, u)[r], f, L);
+                    add(v, cluster.map_shared_rank(mine, u)[r * (HD / 4) + ch], f);
+                }
+                store(r, ch, v, L > 0.f ? 1.f / L : 0.f);
+            }
+            cluster.sync();   // no CTA leaves while another reads its part
+        }
+        return;
+    }
+  }
+}
+
+// Merges the pieces of one item that several CTAs of the wave hold.  One CTA per item; the threads divide the outputs
+// and, where those are few, the pieces.
+template <int HD, int NT, int W>
+__global__ void __launch_bounds__(kMergeThreads) paged_few_merge_kernel(const Paged p, const FewArgs a, unsigned* fault) {
+    constexpr int ROWS = 8 * NT, CH = HD / 4;
+    __shared__ long long s_total, s_before;
+    __shared__ float4 s_o[kMergeThreads];
+    __shared__ float2 s_ml[kMergeThreads];
+    const int b = blockIdx.x / p.NKV, kvh = blockIdx.x - b * p.NKV;
+    if (threadIdx.x < 32) {
+        const long long total = few_sum<ROWS>(p, a, p.n_seqs, fault) * p.NKV;
+        const long long before = few_sum<ROWS>(p, a, b, fault) * p.NKV;
+        if (threadIdx.x == 0) {
+            s_total = total;
+            s_before = before;
+        }
+    }
+    const int tiles = few_tiles<ROWS>(p, a, b, fault);
+    const PagedSeq seq = paged_seq(p, b, fault);
+    __syncthreads();
+    const long long share = few_share(s_total, a.ctas, W), lo = s_before + (long long)kvh * tiles;
+    const int c0 = (int)(lo / share), c1 = tiles > 0 ? (int)((lo + tiles - 1) / share) : c0;
+    pdl_wait();
+    if (c0 == c1) return;   // not ours, or whole: written already
+    const int outs = seq.q * a.G * CH, groups = max(1, kMergeThreads / outs);
+    for (int base = 0; base < outs; base += kMergeThreads) {
+        const int x = base + threadIdx.x % outs, grp = threadIdx.x / outs;
+        const bool on = grp < groups && x < outs;
+        float M = -INFINITY, L = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int r = x / CH, ch = x % CH;
+        if (on) {
+#pragma unroll 4
+            for (int u = c0 + grp; u <= c1; u += groups) {
+                const long long at = ((long long)2 * u + (u == c0 ? 1 : 0)) * ROWS + r;
+                const float2 ml = __ldcg(a.part_ml + at);
+                const float4 y = __ldcg(a.part_o + at * CH + ch);
+                const float t = fmaxf(M, ml.x), base_m = t == -INFINITY ? 0.f : t;
+                const float f = ex2(M - base_m), h = ex2(ml.x - base_m);
+                M = t;
+                L = L * f + ml.y * h;
+                v.x = v.x * f + y.x * h;
+                v.y = v.y * f + y.y * h;
+                v.z = v.z * f + y.z * h;
+                v.w = v.w * f + y.w * h;
+            }
+        }
+        s_o[threadIdx.x] = v;
+        s_ml[threadIdx.x] = make_float2(M, L);
+        __syncthreads();
+        if (on && grp == 0) {
+            float top = -INFINITY;
+            for (int u = 0; u < groups; ++u) top = fmaxf(top, s_ml[u * outs + threadIdx.x].x);
+            L = 0.f;
+            v = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int u = 0; u < groups; ++u) {
+                const float2 ml = s_ml[u * outs + threadIdx.x];
+                const float4 y = s_o[u * outs + threadIdx.x];
+                const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+                L = fmaf(ml.y, f, L);
+                v.x = fmaf(y.x, f, v.x);
+                v.y = fmaf(y.y, f, v.y);
+                v.z = fmaf(y.z, f, v.z);
+                v.w = fmaf(y.w, f, v.w);
+            }
+            const float inv = L > 0.f ? 1.f / L : 0.f;
+            const int tok = r / a.G;
+            __half* dst = a.out + ((long long)(seq.row0 + tok) * a.NH + kvh * a.G + r - tok * a.G) * HD + ch * 4;
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack_half2(v.x * inv, v.y * inv), pack_half2(v.z * inv, v.w * inv));
+        }
+        __syncthreads();
     }
 }
 
-template <int FMT, int HD, int NT, bool BIG>
-cudaError_t launch_as(const Paged& p, const FewArgs& a, int S, unsigned* fault, cudaStream_t st) {
+// How a call's work is divided.
+struct FewPlan {
+    bool wave, big;
+    int S, ctas;
+    size_t bytes;   // of workspace (wave)
+};
+template <int FMT, int HD, int NT>
+FewPlan plan(const Paged& p, int max_kv, bool workspace) {
+    using F = Few<FMT, HD, NT, false>;
+    FewPlan x{};
+    const long long items = (long long)p.n_seqs * p.NKV;
+    const int sms = std::max(1, device_sm_count());
+    const long long slots = (long long)sms * F::kPerSm;
+    // Clusters: one wave of CTAs, each with 64 positions at least (2 FP8 sequences of 4096 over 8 heads: 1 / 2 / 4 / 8
+    // CTAs per item 47 / 27 / 16 / 12 us; 16 of 8192: 117 / 70 / 54 us, and 59 at 8, past one wave).
+    x.S = 1;
+    while (x.S < kMaxSplit && items * x.S * 2 <= slots && max_kv >= x.S * 2 * 64) x.S *= 2;
+    // One wave, where a CTA of a cluster would have more than kLong positions; big CTAs (one per SM, fewer pieces to
+    // merge) where each item is cut into four at least.
+    x.wave = workspace && (long long)max_kv > (long long)x.S * kLong;
+    x.big = x.wave && items * 4 <= sms;
+    x.ctas = x.big ? sms : (int)slots;
+    x.bytes = x.wave ? (size_t)2 * x.ctas * 8 * NT * (HD * 4 + 8) : 0;
+    return x;
+}
+
+template <int FMT, int HD, int NT, bool BIG, bool WAVE>
+cudaError_t launch_as(const Paged& p, const FewArgs& a, const FewPlan& x, unsigned* fault, cudaStream_t st) {
     using F = Few<FMT, HD, NT, BIG>;
-    auto kernel = paged_few_kernel<FMT, HD, NT, BIG>;
+    auto kernel = paged_few_kernel<FMT, HD, NT, BIG, WAVE>;
     static std::atomic<bool> set[kMaxDevices];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev >= kMaxDevices || !set[dev].load(std::memory_order_acquire)) {
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)F::kSmem);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
         if (dev < kMaxDevices) set[dev].store(true, std::memory_order_release);
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)p.n_seqs * p.NKV * S);
+    cfg.gridDim = WAVE ? dim3(x.ctas) : dim3((unsigned)p.n_seqs * p.NKV * x.S);
     cfg.blockDim = dim3(F::kThreads);
     cfg.dynamicSmemBytes = F::kSmem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = S;
+    attr[0].val.clusterDim.x = x.S;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, p, a, fault);
+    cfg.numAttrs = WAVE ? 0 : 1;
+    e = cudaLaunchKernelEx(&cfg, kernel, p, a, fault);
+    if (e != cudaSuccess || !WAVE) return e;
+    return launch_pdl(paged_few_merge_kernel<HD, NT, F::W>, dim3((unsigned)p.n_seqs * p.NKV), dim3(kMergeThreads), 0, st,
+                      p, a, fault);
 }
 
 template <int FMT, int HD, int NT>
-cudaError_t launch(const Paged& p, const FewArgs& a, int max_kv, unsigned* fault, cudaStream_t st) {
-    const long long items = (long long)p.n_seqs * p.NKV;
-    const int sms = device_sm_count();
-    constexpr int W = Few<FMT, HD, NT, true>::W;
-    if (items * kMaxSplit > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-    // Few items over long caches: even 16 CTAs of four warps each leave most of an SM's warps out, so one big CTA
-    // per SM (each warp keeps at least four tiles).
-    if (items * kMaxSplit * 4 < (long long)sms * W && max_kv >= kMaxSplit * W * KT * 4)
-        return launch_as<FMT, HD, NT, true>(p, a, kMaxSplit, fault, st);
-    // Else split until the GPU has several waves of CTAs (sequences differ in length), each warp keeping a tile.
-    const long long slots = (long long)sms * Few<FMT, HD, NT, false>::kPerSm;
-    int S = 1;
-    while (S < kMaxSplit && items * S < 2 * slots && max_kv >= S * 2 * 4 * KT) S *= 2;
-    return launch_as<FMT, HD, NT, false>(p, a, S, fault, st);
+cudaError_t launch(const Paged& p, FewArgs a, int max_kv, void* workspace, size_t bytes, unsigned* fault, cudaStream_t st) {
+    if ((long long)p.n_seqs * p.NKV * kMaxSplit > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+    FewPlan x = plan<FMT, HD, NT>(p, max_kv, true);
+    if (x.wave && (workspace == nullptr || bytes < x.bytes)) x = plan<FMT, HD, NT>(p, max_kv, false);
+    if (!x.wave) return launch_as<FMT, HD, NT, false, false>(p, a, x, fault, st);
+    a.ctas = x.ctas;
+    a.part_o = static_cast<float4*>(workspace);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)2 * x.ctas * 8 * NT * (HD / 4));
+    return x.big ? launch_as<FMT, HD, NT, true, true>(p, a, x, fault, st)
+                 : launch_as<FMT, HD, NT, false, true>(p, a, x, fault, st);
+}
+
+// Calls f<FMT, HD, NT>() for a call's format, head size and rows.
+template <class F>
+auto dispatch(int format, int head_dim, int rows_bound, F&& f) {
+    auto nt = [&](auto fmt, auto hd) {
+        return rows_bound <= 8 ? f(fmt, hd, std::integral_constant<int, 1>()) : f(fmt, hd, std::integral_constant<int, 2>());
+    };
+    auto hd = [&](auto fmt) {
+        return head_dim == 128 ? nt(fmt, std::integral_constant<int, 128>()) : nt(fmt, std::integral_constant<int, 64>());
+    };
+    if (format == AF_KV_F16) return hd(std::integral_constant<int, AF_KV_F16>());
+    if (format == AF_KV_FP8_E4M3) return hd(std::integral_constant<int, AF_KV_FP8_E4M3>());
+    return hd(std::integral_constant<int, AF_KV_INT8>());
 }
 
 }  // namespace
 
+size_t paged_few_workspace(int format, int head_dim, const Paged& p, int rows_bound, int max_kv) {
+    return dispatch(format, head_dim, rows_bound, [&](auto fmt, auto hd, auto nt) {
+        return plan<decltype(fmt)::value, decltype(hd)::value, decltype(nt)::value>(p, max_kv, true).bytes;
+    });
+}
+
 cudaError_t paged_few_launch(int format, int head_dim, const Paged& p, const void* q, long long q_stride, int n_heads,
-                             float scale, int rows_bound, bool alone, int max_kv, void* out, unsigned* fault,
-                             cudaStream_t st) {
+                             float scale, int rows_bound, bool alone, int max_kv, void* out, void* workspace,
+                             size_t workspace_bytes, unsigned* fault, cudaStream_t st) {
     FewArgs a{};
     a.q = static_cast<const __half*>(q);
     a.q_stride = q_stride;
@@ -561,16 +805,10 @@ cudaError_t paged_few_launch(int format, int head_dim, const Paged& p, const voi
     a.G = n_heads / p.NKV;
     a.c = scale * 1.4426950408889634f;
     a.alone = alone ? 1 : 0;
-    auto go = [&](auto fmt, auto hd) {
-        constexpr int f = decltype(fmt)::value, h = decltype(hd)::value;
-        return rows_bound <= 8 ? launch<f, h, 1>(p, a, max_kv, fault, st) : launch<f, h, 2>(p, a, max_kv, fault, st);
-    };
-    auto hd = [&](auto fmt) {
-        return head_dim == 128 ? go(fmt, std::integral_constant<int, 128>()) : go(fmt, std::integral_constant<int, 64>());
-    };
-    if (format == AF_KV_F16) return hd(std::integral_constant<int, AF_KV_F16>());
-    if (format == AF_KV_FP8_E4M3) return hd(std::integral_constant<int, AF_KV_FP8_E4M3>());
-    return hd(std::integral_constant<int, AF_KV_INT8>());
+    return dispatch(format, head_dim, rows_bound, [&](auto fmt, auto hd, auto nt) {
+        return launch<decltype(fmt)::value, decltype(hd)::value, decltype(nt)::value>(p, a, max_kv, workspace,
+                                                                                      workspace_bytes, fault, st);
+    });
 }
 
 }  // namespace af

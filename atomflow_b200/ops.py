@@ -274,7 +274,11 @@ def paged_attention(q, k_pages, v_pages, block_table, kv_len, cu_rows, *, scale=
         out = torch.empty(shape, dtype=_F16, device=q.device)
     else:
         _packed(out, "out", dev, T, nh, hd)
-    check(lib().af_paged_attention(ctypes.byref(kv), ctypes.byref(batch), q.data_ptr(), stride, nh,
-                                   hd ** -0.5 if scale is None else scale, max_q or 0, max_kv or 0, out.data_ptr(),
-                                   torch.cuda.current_stream(dev).cuda_stream), "af_paged_attention")
+    L, k, b = lib(), ctypes.byref(kv), ctypes.byref(batch)
+    # scratch of this call alone, from the stream's allocator: calls on several streams, or in several graphs, share none
+    need = L.af_paged_attention_workspace_bytes(k, b, nh, max_q or 0, max_kv or 0)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    check(L.af_paged_attention(k, b, q.data_ptr(), stride, nh, hd ** -0.5 if scale is None else scale, max_q or 0,
+                               max_kv or 0, out.data_ptr(), ws.data_ptr() if need else None, need,
+                               torch.cuda.current_stream(dev).cuda_stream), "af_paged_attention")
     return out

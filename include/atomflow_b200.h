@@ -371,9 +371,15 @@ af_status af_gemv_chain_fast(const af_chain_op* ops, int n_ops, void* workspace,
  *                       FP16 [n_tokens][NH][HD], NH % NKV == 0.  max_rows and
  *                       max_kv are the host's bounds on a sequence's rows and
  *                       positions (0: not known): they choose how the work is
- *                       split, never the result's meaning.
- * q, out, qkv, q_out, k_out, v_out 16-byte aligned.  No workspace; no
- * allocation. */
+ *                       split, never the result's meaning.  A sequence of more
+ *                       rows than a non-zero max_rows may be left out (then
+ *                       AF_FAULT_PAGED).  workspace (16-byte aligned, any
+ *                       contents) is optional: with the bytes that
+ *                       af_paged_attention_workspace_bytes names for the same
+ *                       bounds (0: none of use), long caches of few rows are cut
+ *                       evenly over the whole GPU instead of over clusters.
+ *                       Calls that share a workspace must not overlap.
+ * q, out, qkv, q_out, k_out, v_out 16-byte aligned.  No allocation. */
 typedef enum af_kv_format {
     AF_KV_F16 = 0,
     AF_KV_FP8_E4M3 = 1,
@@ -401,8 +407,11 @@ af_status af_paged_kv_write(const af_paged_kv* kv, const af_paged_batch* batch, 
                             void* stream);
 af_status af_paged_kv_read(const af_paged_kv* kv, const af_paged_batch* batch, void* k_out, void* v_out,
                            void* stream);
+size_t af_paged_attention_workspace_bytes(const af_paged_kv* kv, const af_paged_batch* batch, int n_heads,
+                                          int max_rows, int max_kv);
 af_status af_paged_attention(const af_paged_kv* kv, const af_paged_batch* batch, const void* q, int64_t q_stride,
-                             int n_heads, float scale, int max_rows, int max_kv, void* out, void* stream);
+                             int n_heads, float scale, int max_rows, int max_kv, void* out, void* workspace,
+                             size_t workspace_bytes, void* stream);
 
 /* -------------------------------------------------------- decode engine ---
  * A whole greedy decode step of a model in the reference's .bin format

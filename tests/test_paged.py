@@ -102,7 +102,7 @@ def _calls(kv, b):
     L, R = lib(), ctypes.byref
     return [L.af_paged_kv_write(R(kv), R(b), 4096, 8 * 128, 4, None, None, 0, None, None),
             L.af_paged_kv_read(R(kv), R(b), 4096, 4096, None),
-            L.af_paged_attention(R(kv), R(b), 4096, 4 * 128, 4, 0.1, 0, 0, 4096, None)]
+            L.af_paged_attention(R(kv), R(b), 4096, 4 * 128, 4, 0.1, 0, 0, 4096, None, 0, None)]
 
 
 @pytest.mark.parametrize("over,status", [
@@ -138,8 +138,8 @@ def test_bad_rows_are_refused():
     def write(qkv=4096, stride=8 * 128, heads=4, cos=None, sin=None, max_seq=0, q=None):
         return L.af_paged_kv_write(R(kv), R(b), qkv, stride, heads, cos, sin, max_seq, q, None)
 
-    def attend(q=4096, stride=4 * 128, heads=4, scale=0.1, rows=0, kvb=0, out=4096):
-        return L.af_paged_attention(R(kv), R(b), q, stride, heads, scale, rows, kvb, out, None)
+    def attend(q=4096, stride=4 * 128, heads=4, scale=0.1, rows=0, kvb=0, out=4096, ws=None):
+        return L.af_paged_attention(R(kv), R(b), q, stride, heads, scale, rows, kvb, out, ws, 0, None)
 
     assert write(qkv=None) == write(qkv=4104) == write(stride=8 * 128 - 8) == write(stride=8 * 128 + 4) == 1
     assert write(heads=-1) == write(cos=4096, q=4096, max_seq=8) == write(cos=4096, sin=4096, q=4096) == 1
@@ -147,7 +147,7 @@ def test_bad_rows_are_refused():
     assert write(cos=4104, sin=4096, max_seq=8, q=4096) == 1
     assert attend(q=None) == attend(out=None) == attend(q=4104) == attend(out=4104) == 1
     assert attend(stride=4 * 128 - 8) == attend(stride=4 * 128 + 4) == attend(heads=3) == attend(heads=0) == 1
-    assert attend(rows=-1) == attend(kvb=-1) == 1
+    assert attend(rows=-1) == attend(kvb=-1) == attend(ws=4104) == 1
     for bad in (0.0, -1.0, float("nan"), float("inf")):
         assert attend(scale=bad) == 1
     assert L.af_paged_kv_read(R(kv), R(b), None, 4096, None) == L.af_paged_kv_read(R(kv), R(b), 4096, 4104, None) == 1
