@@ -27,9 +27,10 @@
 //     loaded in that order).  8-bit V pairs positions by byte permutes.
 //   * INT8 K is used as 1024 + code + 128, the byte as an FP16 mantissa; the
 //     accumulator starts at -1152 sum(q), which takes the offset out again.
-//   * K's scale multiplies S in FP32; V is scaled into FP16 (the values
-//     af_paged_kv_read returns), as P has no room for a scale that may be
-//     subnormal in FP16.  P is rounded to FP16.
+//   * K's scale multiplies S in FP32.  V's goes into P: the weight P v_scale r is
+//     rounded to FP16 once, r a power of two that brings the scales met so far to
+//     about 1 (raised scales rescale O as a raised maximum does), and V's codes
+//     are exact.  (Scaling V itself took 32 of 404 instructions per tile.)
 //   * Warps and CTAs merge in a fixed order: the same bits every time.
 //   * The loop is bound by issue slots as much as by DRAM: 8 warps per SM (two per
 //     scheduler) issued in 45% of the cycles and read the cache at 3.6 TB/s, so
@@ -39,6 +40,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <climits>
 #include <type_traits>
 
 #include "af_paged.cuh"
@@ -47,9 +49,12 @@ namespace af {
 namespace {
 
 constexpr int kMaxSplit = 8;
-constexpr int kMergeThreads = 512;
+constexpr int kMergeThreads = 512;  // at most
 constexpr int KT = 16;             // positions of a tile
-constexpr int kLong = 512;         // positions per CTA of a cluster past which the work is cut into one wave
+constexpr int kLong = 2560;        // positions per CTA of a cluster past which the work is cut into one wave (16 FP16
+                                   // sequences of 4096 over 8 heads: clusters of 2 44 us, wave 48; 4 FP8 of 32768:
+                                   // clusters of 8 71 us, wave 54)
+constexpr float kRise = 16.f;      // V's scale times r past which r moves: P v_scale r <= 2^8 * 2^4
 constexpr float kGrow = 8.f;       // log2 of the growth of a score over the maximum that moves it
 
 // NT: 8-row column tiles; BIG: one CTA per SM with all its warps, else CTAs of four warps.
@@ -87,8 +92,11 @@ struct FewArgs {
     int NH, G;
     float c;       // scale * log2(e)
     int alone;     // no other kernel takes the sequences of too many rows: record them
-    float4* part_o;   // one wave: partial O [2 ctas][ROWS][HD], m and l [2 ctas][ROWS]
+    // one wave: partial O [2 ctas][ROWS][HD], m and l [2 ctas][ROWS], and for each CTA the item that begins in it and
+    // goes on in the next ones: {first row, kv head, pieces (0: no such item), rows}
+    float4* part_o;
     float2* part_ml;
+    int4* part_head;
     int ctas;
 };
 
@@ -149,42 +157,70 @@ __device__ __forceinline__ int few_tiles(const Paged& p, const FewArgs& a, int b
     }
     return max(1, (s.kv + KT - 1) / KT);
 }
-// By one whole warp: tiles of one head of sequences [0, n).
+// A CTA's piece of the wave: tiles [lo, hi) of the row of all, beginning in sequence b (-1: nothing), whose first tile
+// is `first`.  The item that begins in the piece and goes on ends `tiles - 1` later, in CTA (its last tile) / share,
+// or, where all sequences are as long (`even` > 0), after `even` CTAs: each item is then cut into that many pieces at
+// its own borders, so that no CTA has parts of two.
+struct FewPiece {
+    long long lo, hi, first, share;
+    int b, even;
+};
+// By one whole warp.
 template <int ROWS>
-__device__ long long few_sum(const Paged& p, const FewArgs& a, int n, unsigned* fault) {
-    long long t = 0;
-    for (int b = threadIdx.x & 31; b < n; b += 32) t += few_tiles<ROWS>(p, a, b, fault);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) t += __shfl_xor_sync(0xffffffffu, t, x);
-    return t;
-}
-// By one whole warp: the sequence that holds tile u of the row (u < all tiles), and its first tile.
-template <int ROWS>
-__device__ int few_find(const Paged& p, const FewArgs& a, long long u, long long& first, unsigned* fault) {
+__device__ FewPiece few_piece(const Paged& p, const FewArgs& a, int cta, int W, unsigned* fault) {
     const int lane = threadIdx.x & 31;
+    const unsigned all = 0xffffffffu;
+    long long heads = 0;                 // tiles of one head of every sequence
+    int low = INT_MAX, high = 0, t0 = 0; // t0: of sequence `lane`, kept where that is all there is
+    for (int b = lane; b < p.n_seqs; b += 32) {
+        const int t = few_tiles<ROWS>(p, a, b, fault);
+        if (b == lane) t0 = t;
+        heads += t;
+        low = min(low, t);
+        high = max(high, t);
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) heads += __shfl_xor_sync(all, heads, x);
+    low = __reduce_min_sync(all, low);
+    high = __reduce_max_sync(all, high);
+    FewPiece r{0, 0, 0, 1, -1, 0};
+    const long long total = heads * p.NKV, items = (long long)p.n_seqs * p.NKV;
+    if (total == 0) return r;
+    if (low == high && items <= a.ctas) {
+        const int k = max(1, (int)min((long long)(a.ctas / items), (long long)low / (2 * W)));   // two tiles per warp
+        const int item = cta / k, piece = cta - item * k;
+        if (item >= items) return r;
+        r.even = k;
+        r.b = item / p.NKV;
+        r.first = (long long)r.b * p.NKV * low;
+        r.lo = (long long)item * low + (long long)low * piece / k;
+        r.hi = (long long)item * low + (long long)low * (piece + 1) / k;
+        return r;
+    }
+    r.share = max((total + a.ctas - 1) / a.ctas, (long long)2 * W);
+    r.lo = cta * r.share;
+    r.hi = min(total, r.lo + r.share);
+    if (r.lo >= r.hi) return r;
     long long seen = 0;
     for (int b0 = 0; b0 < p.n_seqs; b0 += 32) {
-        const long long t = b0 + lane < p.n_seqs ? (long long)few_tiles<ROWS>(p, a, b0 + lane, fault) * p.NKV : 0;
+        const long long t =
+            (long long)(b0 == 0 ? t0 : b0 + lane < p.n_seqs ? few_tiles<ROWS>(p, a, b0 + lane, fault) : 0) * p.NKV;
         long long inc = t;
 #pragma unroll
         for (int x = 1; x < 32; x <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, inc, x);
+            const long long y = __shfl_up_sync(all, inc, x);
             if (lane >= x) inc += y;
         }
-        const unsigned who = __ballot_sync(0xffffffffu, u >= seen + inc - t && u < seen + inc);
+        const unsigned who = __ballot_sync(all, r.lo >= seen + inc - t && r.lo < seen + inc);
         if (who != 0) {
             const int src = __ffs(who) - 1;
-            first = seen + __shfl_sync(0xffffffffu, inc - t, src);
-            return b0 + src;
+            r.first = seen + __shfl_sync(all, inc - t, src);
+            r.b = b0 + src;
+            return r;
         }
-        seen += __shfl_sync(0xffffffffu, inc, 31);
+        seen += __shfl_sync(all, inc, 31);
     }
-    return -1;
-}
-// Tiles per CTA: an equal share, at least two per warp.
-__device__ __forceinline__ long long few_share(long long total, int ctas, int W) {
-    const long long u = (total + ctas - 1) / ctas;
-    return u < 2 * W ? 2 * W : u;
+    return r;
 }
 
 template <int FMT, int HD, int NT, bool BIG, bool WAVE>
@@ -199,29 +235,25 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     int S = 1, rank = 0, b, kvh, t0, t1;
     PagedSeq seq;
-    long long u0 = 0, u1 = 0, first = 0;     // one wave: this CTA's tiles; first tile of sequence b
+    long long u0 = 0, u1 = 0, first = 0, share = 1;   // one wave: this CTA's piece
+    int even = 0;
     if constexpr (WAVE) {
         pdl_launch_dependents();             // every CTA is resident: the merge may line up behind them
-        __shared__ long long s_first, s_u0, s_u1;
-        __shared__ int s_b;
+        __shared__ FewPiece s_piece;
         if (warp == 0) {
-            const long long total = few_sum<ROWS>(p, a, p.n_seqs, fault) * p.NKV;
-            const long long share = few_share(total, a.ctas, W);
-            const long long lo = (long long)blockIdx.x * share, hi = min(total, lo + share);
-            long long f = 0;
-            const int at = lo < hi ? few_find<ROWS>(p, a, lo, f, fault) : -1;
+            const FewPiece x = few_piece<ROWS>(p, a, blockIdx.x, W, fault);
             if (lane == 0) {
-                s_u0 = lo;
-                s_u1 = hi;
-                s_first = f;
-                s_b = at;
+                s_piece = x;
+                a.part_head[blockIdx.x] = make_int4(0, 0, 0, 0);
             }
         }
         __syncthreads();
-        b = s_b;
-        u0 = s_u0;
-        u1 = s_u1;
-        first = s_first;
+        b = s_piece.b;
+        u0 = s_piece.lo;
+        u1 = s_piece.hi;
+        first = s_piece.first;
+        share = s_piece.share;
+        even = s_piece.even;
         if (b < 0) return;
     } else {
         cg::cluster_group cluster = cg::this_cluster();
@@ -259,12 +291,19 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
     struct Pages {
         int lo, hi;
     };
+    const int* table = p.table + paged_table_at(b, p.table_stride, 0, 0);
+    auto page_of = [&](int pos) {
+        const int page = __ldg(table + (pos >> p.page_shift));
+        if (paged_page_ok(page, p.n_pages)) return page;
+        atomicOr(fault, (unsigned)AF_FAULT_PAGED);
+        return -1;
+    };
     auto find = [&](int j) {
         Pages x{-1, -1};
         const int pos = (t0 + warp + W * j) * KT;
         if (j < n && pos < end) {
-            x.lo = paged_page(p, b, pos, fault);
-            x.hi = p.page_shift > 3 ? x.lo : pos + 8 < end ? paged_page(p, b, pos + 8, fault) : -1;
+            x.lo = page_of(pos);
+            x.hi = p.page_shift > 3 ? x.lo : pos + 8 < end ? page_of(pos + 8) : -1;
         }
         return x;
     };
@@ -282,10 +321,9 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
         k_to[i] = F::at(row_of + i * RPI, lane % F::kCh, false);
         v_to[i] = F::kHalf + F::at(row_of + i * RPI, lane % F::kCh, true);
     }
-    auto issue = [&](int j, Pages pg) {
+    auto issue = [&](int j, uint32_t stage, Pages pg) {
         if (j < n) {
             const int pos = (t0 + warp + W * j) * KT;
-            const uint32_t stage = ring + (j % F::kStages) * (2 * F::kHalf);
             const long long lo = paged_at(p, max(pg.lo, 0), pos, 0, F::kRow);
             const long long hi = p.page_shift > 3 ? lo + 8 * row_bytes : paged_at(p, max(pg.hi, 0), pos, 0, F::kRow);
             if ((pg.lo | pg.hi) >= 0 && pos + KT <= end) {
@@ -308,11 +346,12 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
         cp_async_commit();
     };
     // Scales of tile j: lane l < 16 K's of position l, lane 16 + l V's.
+    const __half* sc_lane = (lane < 16 ? p.ks : p.vs) + kvh;
     auto scales = [&](int j, Pages pg) {
         __half x = __float2half_rn(0.f);
         if constexpr (FMT != AF_KV_F16) {
             const int pos = (t0 + warp + W * j) * KT + (lane & 15), page = lane & 8 ? pg.hi : pg.lo;
-            if (page >= 0 && pos < end) x = __ldg((lane < 16 ? p.ks : p.vs) + paged_scale(p, page, pos, kvh));
+            if (page >= 0 && pos < end) x = __ldg(sc_lane + paged_scale(p, page, pos, 0));
         }
         return x;
     };
@@ -324,7 +363,7 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
     for (int j = 0; j < D; ++j) {
         const Pages pg = next;
         next = find(j + 1);
-        issue(j, pg);
+        issue(j, ring + j * (2 * F::kHalf), pg);
         sc_ring[j] = scales(j, pg);
     }
 
@@ -380,19 +419,25 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[t][nt][e] = 0.f;
 
+    float r = 1.f;                                   // V's scales are about 1 / r
+    uint32_t stage = ring, to = ring + D * (2 * F::kHalf);
+    const uint32_t ring_end = ring + F::kStages * (2 * F::kHalf);
     for (int j = 0; j < n; ++j) {
         // the stage that tile j + D goes into was read in the last iteration
         __syncwarp();
         const Pages pg = next;
         next = find(j + D + 1);
-        issue(j + D, pg);
+        issue(j + D, to, pg);
         const __half sc_new = scales(j + D, pg), sc = sc_ring[0];
 #pragma unroll
         for (int x = 0; x + 1 < D; ++x) sc_ring[x] = sc_ring[x + 1];
         sc_ring[D - 1] = sc_new;
         cp_async_wait<D>();
         __syncwarp();
-        const uint32_t ks = ring + (j % F::kStages) * (2 * F::kHalf), vs = ks + F::kHalf;
+        const uint32_t ks = stage, vs = ks + F::kHalf;
+        to = stage;
+        stage += 2 * F::kHalf;
+        if (stage == ring_end) stage = ring;
         const int pos0 = (t0 + warp + W * j) * KT;
 
         float s[NT][4];
@@ -431,12 +476,16 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
             }
         }
         // scores in the exponent's base 2; positions a row does not see: -inf
-        float k0 = a.c, k1 = a.c;
-        if constexpr (FMT != AF_KV_F16) {
-            k0 *= __half2float(__shfl_sync(0xffffffffu, sc, g));
-            k1 *= __half2float(__shfl_sync(0xffffffffu, sc, g + 8));
-        }
+        float k0 = a.c, k1 = a.c, v0 = 0.f, v1 = 0.f;
         bool up = false;
+        if constexpr (FMT != AF_KV_F16) {
+            const float x = __half2float(sc);
+            k0 *= __shfl_sync(0xffffffffu, x, g);
+            k1 *= __shfl_sync(0xffffffffu, x, g + 8);
+            v0 = __shfl_sync(0xffffffffu, x, 16 + g);
+            v1 = __shfl_sync(0xffffffffu, x, 24 + g);
+            up = fmaxf(fabsf(v0), fabsf(v1)) * r > kRise;
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -461,6 +510,17 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
                 up |= t > m[nt][e] + kGrow;
             }
         if (__any_sync(0xffffffffu, up)) {
+            float q = 1.f;                           // r's change
+            if constexpr (FMT != AF_KV_F16) {
+                float t = fminf(fmaxf(fabsf(v0), fabsf(v1)), 65504.f);
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
+                if (t * r > kRise || (r == 1.f && t > 0.f)) {   // (an FP16 scale's exponent: 2^-24 .. 2^16)
+                    const float to_one = __uint_as_float((254u << 23) - (__float_as_uint(t) & 0x7f800000u));
+                    q = to_one / r;
+                    r = to_one;
+                }
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -468,9 +528,10 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
                     float t = fmaxf(m[nt][e], fmaxf(s[nt][e], s[nt][2 + e]));
 #pragma unroll
                     for (int x = 4; x < 32; x <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
-                    const float f = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - t);
+                    float f = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - t);
                     m[nt][e] = t;
                     l[nt][e] *= f;
+                    f *= q;
 #pragma unroll
                     for (int x = 0; x < MT; ++x) {
                         o[x][nt][e] *= f;
@@ -478,6 +539,8 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
                     }
                 }
         }
+        v0 *= r;
+        v1 *= r;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -487,7 +550,7 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
                 for (int h = 0; h < 2; ++h) {
                     const float w = ex2(s[nt][2 * h + e] - base);
                     l[nt][e] += w;
-                    s[nt][2 * h + e] = w;
+                    s[nt][2 * h + e] = FMT == AF_KV_F16 ? w : w * (h ? v1 : v0);
                 }
             }
         uint32_t pb[NT][2];
@@ -505,9 +568,6 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
                 for (int nt = 0; nt < NT; ++nt) mma16816(o[t][nt], v[0], v[1], v[2], v[3], pb[nt][0], pb[nt][1]);
             }
         } else {
-            const int k = 2 * c;
-            const __half2 s01 = __halves2half2(__shfl_sync(0xffffffffu, sc, 16 + k), __shfl_sync(0xffffffffu, sc, 17 + k));
-            const __half2 s89 = __halves2half2(__shfl_sync(0xffffffffu, sc, 24 + k), __shfl_sync(0xffffffffu, sc, 25 + k));
 #pragma unroll
             for (int d = 0; d < HD / 32; ++d) {   // the lane's dims: 32 d + 4 g + 0..3
                 const uint32_t at = vs + (v_at ^ (d * 32));
@@ -519,10 +579,6 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
                     uint32_t a0, a1, a2, a3;
                     kv_unpack4<FMT>(__byte_perm(w0, w1, h ? 0x7362 : 0x5140), a0, a1);
                     kv_unpack4<FMT>(__byte_perm(w8, w9, h ? 0x7362 : 0x5140), a2, a3);
-                    a0 = mul_half2(a0, s01);
-                    a1 = mul_half2(a1, s01);
-                    a2 = mul_half2(a2, s89);
-                    a3 = mul_half2(a3, s89);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) mma16816(o[2 * d + h][nt], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
                 }
@@ -533,24 +589,25 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
     __syncthreads();   // every ring is idle: the warps' parts go there, FP32 [warp][row][HD]
     float* part = reinterpret_cast<float*>(smem);
     static_assert((size_t)(W + 1) * ROWS * HD * 4 <= F::kSmem, "parts fit");
+    const float back = 1.f / r;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const int r = nt * 8 + 2 * c + e;
+            const int row = nt * 8 + 2 * c + e;
             float t = l[nt][e];
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) t += __shfl_xor_sync(0xffffffffu, t, x);
             if (g == 0) {
-                s_m[warp][r] = m[nt][e];
-                s_l[warp][r] = t;
+                s_m[warp][row] = m[nt][e];
+                s_l[warp][row] = t;
             }
 #pragma unroll
             for (int t2 = 0; t2 < MT; ++t2)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int d = FMT == AF_KV_F16 ? 16 * t2 + g + 8 * h : 32 * (t2 >> 1) + 4 * g + 2 * (t2 & 1) + h;
-                    part[(warp * ROWS + r) * HD + d] = o[t2][nt][2 * h + e];
+                    part[(warp * ROWS + row) * HD + d] = o[t2][nt][2 * h + e] * back;
                 }
         }
     __syncthreads();
@@ -594,6 +651,9 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
         }
     }
     if constexpr (WAVE) {
+        if (t0 == 0 && t1 < tiles && threadIdx.x == 0)
+            a.part_head[blockIdx.x] =
+                make_int4(seq.row0, kvh, even > 0 ? even : (int)((u0 + tiles - 1) / share) - (int)blockIdx.x + 1, rows);
         u0 += t1 - t0;
         if (u0 >= u1) return;
         if (u0 - first >= (long long)tiles * p.NKV) {   // on to the next sequence that is ours
@@ -629,32 +689,19 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
   }
 }
 
-// Merges the pieces of one item that several CTAs of the wave hold.  One CTA per item; the threads divide the outputs
-// and, where those are few, the pieces.
-template <int HD, int NT, int W>
-__global__ void __launch_bounds__(kMergeThreads) paged_few_merge_kernel(const Paged p, const FewArgs a, unsigned* fault) {
+// Merges the pieces of the item that begins in CTA blockIdx.x of the wave and goes on in the next ones.  The threads
+// divide the outputs and, where those are few, the pieces.
+template <int HD, int NT>
+__global__ void __launch_bounds__(kMergeThreads) paged_few_merge_kernel(const FewArgs a) {
     constexpr int ROWS = 8 * NT, CH = HD / 4;
-    __shared__ long long s_total, s_before;
     __shared__ float4 s_o[kMergeThreads];
     __shared__ float2 s_ml[kMergeThreads];
-    const int b = blockIdx.x / p.NKV, kvh = blockIdx.x - b * p.NKV;
-    if (threadIdx.x < 32) {
-        const long long total = few_sum<ROWS>(p, a, p.n_seqs, fault) * p.NKV;
-        const long long before = few_sum<ROWS>(p, a, b, fault) * p.NKV;
-        if (threadIdx.x == 0) {
-            s_total = total;
-            s_before = before;
-        }
-    }
-    const int tiles = few_tiles<ROWS>(p, a, b, fault);
-    const PagedSeq seq = paged_seq(p, b, fault);
-    __syncthreads();
-    const long long share = few_share(s_total, a.ctas, W), lo = s_before + (long long)kvh * tiles;
-    const int c0 = (int)(lo / share), c1 = tiles > 0 ? (int)((lo + tiles - 1) / share) : c0;
     pdl_wait();
-    if (c0 == c1) return;   // not ours, or whole: written already
-    const int outs = seq.q * a.G * CH, groups = max(1, kMergeThreads / outs);
-    for (int base = 0; base < outs; base += kMergeThreads) {
+    const int4 head = __ldcg(a.part_head + blockIdx.x);
+    if (head.z == 0) return;
+    const int kvh = head.y, c0 = blockIdx.x, c1 = c0 + head.z - 1;
+    const int outs = head.w * CH, groups = max(1, (int)blockDim.x / outs);
+    for (int base = 0; base < outs; base += blockDim.x) {
         const int x = base + threadIdx.x % outs, grp = threadIdx.x / outs;
         const bool on = grp < groups && x < outs;
         float M = -INFINITY, L = 0.f;
@@ -696,7 +743,7 @@ __global__ void __launch_bounds__(kMergeThreads) paged_few_merge_kernel(const Pa
             }
             const float inv = L > 0.f ? 1.f / L : 0.f;
             const int tok = r / a.G;
-            __half* dst = a.out + ((long long)(seq.row0 + tok) * a.NH + kvh * a.G + r - tok * a.G) * HD + ch * 4;
+            __half* dst = a.out + ((long long)(head.x + tok) * a.NH + kvh * a.G + r - tok * a.G) * HD + ch * 4;
             *reinterpret_cast<uint2*>(dst) = make_uint2(pack_half2(v.x * inv, v.y * inv), pack_half2(v.z * inv, v.w * inv));
         }
         __syncthreads();
@@ -724,8 +771,8 @@ FewPlan plan(const Paged& p, int max_kv, bool workspace) {
     // merge) where each item is cut into four at least.
     x.wave = workspace && (long long)max_kv > (long long)x.S * kLong;
     x.big = x.wave && items * 4 <= sms;
-    x.ctas = x.big ? sms : (int)slots;
-    x.bytes = x.wave ? (size_t)2 * x.ctas * 8 * NT * (HD * 4 + 8) : 0;
+    x.ctas = (int)(x.big ? sms : slots);   // as many as the GPU holds
+    x.bytes = x.wave ? (size_t)x.ctas * (2 * 8 * NT * (HD * 4 + 8) + 16) : 0;
     return x;
 }
 
@@ -755,8 +802,7 @@ cudaError_t launch_as(const Paged& p, const FewArgs& a, const FewPlan& x, unsign
     cfg.numAttrs = WAVE ? 0 : 1;
     e = cudaLaunchKernelEx(&cfg, kernel, p, a, fault);
     if (e != cudaSuccess || !WAVE) return e;
-    return launch_pdl(paged_few_merge_kernel<HD, NT, F::W>, dim3((unsigned)p.n_seqs * p.NKV), dim3(kMergeThreads), 0, st,
-                      p, a, fault);
+    return launch_pdl(paged_few_merge_kernel<HD, NT>, dim3(x.ctas), dim3(BIG ? kMergeThreads : 256), 0, st, a);
 }
 
 template <int FMT, int HD, int NT>
@@ -768,6 +814,7 @@ cudaError_t launch(const Paged& p, FewArgs a, int max_kv, void* workspace, size_
     a.ctas = x.ctas;
     a.part_o = static_cast<float4*>(workspace);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)2 * x.ctas * 8 * NT * (HD / 4));
+    a.part_head = reinterpret_cast<int4*>(a.part_ml + (size_t)2 * x.ctas * 8 * NT);
     return x.big ? launch_as<FMT, HD, NT, true, true>(p, a, x, fault, st)
                  : launch_as<FMT, HD, NT, false, true>(p, a, x, fault, st);
 }

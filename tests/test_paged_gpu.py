@@ -9,7 +9,10 @@ W = sum p_j |v_j| and w_j = exp(s_j - max s) the weights before the division:
     is subnormal in FP16, relative to a largest weight of at least 1:
     2^-25 sum |v_j| / sum w_j
   * 8-bit caches: K and V are used as FP16 (code * scale, one rounding): 2^-11 W
-    for V; for K a score error of at most 2^-11 scale sum_d |q_d k_d|
+    for V; for K a score error of at most 2^-11 scale sum_d |q_d k_d|.  (The path
+    of few rows is more exact there: it scales S in FP32, and V's scale, brought
+    to about 1 for the largest, goes into the one rounding of P; a weight that is
+    then subnormal is off by 2^-25 of the largest scale's: 2^-25 n max|v| / sum w_j.)
   * scores, sums and products in FP32: a score error of 2^-24 (HD / 16 + 8) scale
     sum |q_d k_d| and of 2^-22 relative in each exponential's argument and
     value, and 2^-19 W for the sums (up to 2^4 partial orders, truncating
@@ -148,6 +151,8 @@ def attention_f64(c, q, scale, b, row):
     seen = (~hidden).double()
     tol = (2.0 ** -11 * out.abs() + 2.0 ** -25 + W * ((2 if quant else 1) * 2.0 ** -11 + torch.expm1(2 * d) + 2.0 ** -19) +
            2.0 ** -25 * (seen @ v.abs()) / total.clamp(min=1e-300).clamp(min=1.0))
+    if quant:
+        tol = tol + 2.0 ** -25 * (seen @ v.abs().amax(-1, keepdim=True)) / total.clamp(min=1e-300).clamp(min=1.0)
     empty = total == 0
     out, tol = out.masked_fill(empty, 0.0), tol.masked_fill(empty, 0.0)
     return out.transpose(0, 1), tol.transpose(0, 1)
