@@ -15,9 +15,13 @@
 //     coordinate outside the tensor, which reads as zeros.  8-bit codes land in a
 //     staging ring, and warps 12-15 multiply them by their scales into FP16 slots
 //     (the values af_paged_kv_read returns).
-//   * V rows past the sequence's end would meet weights of zero, but what lies there
-//     may be NaN: warps 12-15 put zeros in their place.  (K rows there give scores
-//     that are masked.)
+//   * V at positions that a row does not see (behind it in its own chunk, or past the
+//     end) meets weights of zero; where it is an infinity or NaN the product would be
+//     NaN.  Warps 12-15 put zeros in the place of such values, and the epilogue adds
+//     them back for the rows that do see them.  (K there gives scores that are
+//     masked.)
+//   * The output goes through shared memory (Q's place) to whole rows per half warp:
+//     rows written by a thread each cost the LSU eight times the wavefronts.
 //   * Warp 8 issues the MMAs.  S of both row tiles and O of both fill the 512
 //     TMEM columns; P (FP16) overwrites the S it came from and is the A operand
 //     of the second product straight from TMEM.  The order PV(0, j), QK(0, j+1),
@@ -226,6 +230,66 @@ __device__ __forceinline__ bool tc_wait(const uint64_t* bar, uint32_t parity, vo
     return false;
 }
 
+// V's element as the attention sees it.
+template <int FMT, int HD>
+__device__ float v_value(const Paged& p, int b, int pos, int kvh, int d, unsigned* fault) {
+    const int page = paged_page(p, b, pos, fault);
+    if (page < 0) return 0.f;
+    const uint8_t* at = p.v + paged_at(p, page, pos, kvh, HD * KvFormat<FMT>::kBytes);
+    if constexpr (FMT == AF_KV_F16) return __half2float(reinterpret_cast<const __half*>(at)[d]);
+    const float s = __half2float(p.vs[paged_scale(p, page, pos, kvh)]);
+    if constexpr (FMT == AF_KV_INT8) return (float)reinterpret_cast<const int8_t*>(at)[d] * s;
+    return (float)reinterpret_cast<const __nv_fp8_e4m3*>(at)[d] * s;
+}
+// Adds to a row's output (FP16, or FP32 in a cluster's part) what was taken out of V at positions [from, to).  Rare and
+// out of line: the row's outputs are read back.
+template <int FMT, int HD>
+__device__ __noinline__ void add_mended(const Paged& p, int b, int kvh, int from, int to, __half* dst, float* part, int r,
+                                        unsigned* fault) {
+#pragma unroll 1
+    for (int pos = from; pos < to; ++pos)
+#pragma unroll 1
+        for (int d = 0; d < HD; ++d) {
+            const float x = v_value<FMT, HD>(p, b, pos, kvh, d, fault);
+            if (fabsf(x) < 65520.f) continue;
+            if (part != nullptr) part[((d >> 2) ^ (r & (HD / 4 - 1))) * 4 + (d & 3)] += x;
+            else dst[d] = __float2half_rn(__half2float(dst[d]) + x);
+        }
+}
+// Puts zeros in the place of infinities and NaN in a pair of FP16 values; whether there were any.
+__device__ __forceinline__ bool mend_half2(uint32_t& v) {
+    const bool lo = (v & 0x7c00u) == 0x7c00u, hi = (v & 0x7c000000u) == 0x7c000000u;
+    if (lo) v &= 0xffff0000u;
+    if (hi) v &= 0x0000ffffu;
+    return lo | hi;
+}
+__device__ __forceinline__ bool mend_chunk(uint4& v) {
+    const bool a = mend_half2(v.x), b = mend_half2(v.y), c = mend_half2(v.z), d = mend_half2(v.w);
+    return a | b | c | d;
+}
+
+// The same for the chunks of a tile of codes that thread i has just converted, in rows from `from` on.
+template <int HD>
+__device__ __noinline__ bool mend_rows(unsigned char* tile, int i, int from) {
+    constexpr int C8 = HD / 16, RC = 128 / C8;
+    bool mended = false;
+#pragma unroll 1
+    for (int r = i / C8; r < kTile; r += RC) {
+        if (r < from) continue;
+#pragma unroll 1
+        for (int e = 0; e < 2; ++e) {
+            const int ch = 2 * (i % C8) + e;
+            uint4* at = reinterpret_cast<uint4*>(tile + (ch >> 3) * (kTile * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
+            uint4 y = *at;
+            if (mend_chunk(y)) {
+                *at = y;
+                mended = true;
+            }
+        }
+    }
+    return mended;
+}
+
 template <int FMT, int HD>
 __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p, const TcArgs a,
                                                                    const __grid_constant__ CUtensorMap k_map,
@@ -237,6 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
     __shared__ __align__(8) Bars bars;
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_abort;
+    __shared__ volatile int s_mended;                // V had infinities or NaN where some row does not look
     __shared__ int s_item[2];                        // sequence, row tile pair
     __shared__ __half s_scale[2][2][kTile];          // two tiles' scales: K's, V's
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -276,6 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
             s_item[0] = fb;
             s_item[1] = ft;
             s_abort = 0;
+            s_mended = 0;
         }
     }
     if (warp == kMmaWarp) {
@@ -318,8 +384,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
     const int tiles = (end + kTile - 1) / kTile;
     const int t0 = (int)((long long)tiles * rank / S), t1 = (int)((long long)tiles * (rank + 1) / S);
     const int n = t1 - t0;
-    // tiles from first_masked on hold positions that some row does not see
-    const int first_masked = max(0, max(0, ctx + row_base / a.G + 1) / kTile - t0);
+    // positions that every row sees; tiles from first_masked on hold others
+    const int all_see = max(0, ctx + row_base / a.G + 1), first_masked = max(0, all_see / kTile - t0);
     unsigned char* q_s = smem;
     unsigned char* ring = smem + Sh::kRing;
     // the cluster merge's parts, in the buffers once they are idle: FP32 O [256][HD], then m and l [256]
@@ -354,15 +420,26 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
                 cp_async_wait<0>();
                 fence_async_smem();
                 mbar_arrive(smem_u32(&bars.q_full));
-                // V tiles with masked positions come by way of these warps: zeros past the end
+                // V tiles with masked positions come by way of these warps: zeros past the end and in the place of
+                // infinities and NaN
+                bool mended = false;
                 for (int j = first_masked; j < n; ++j) {
                     const int slot = (2 * j + 1) % Sh::kSlots;
                     tc_wait(&bars.raw_full[j - first_masked], 0, &s_abort, fault);
-                    const int first = max(0, end - (t0 + j) * kTile);
+                    const int pos0 = (t0 + j) * kTile, from = max(0, all_see - pos0), left = end - pos0;
                     unsigned char* v = ring + slot * Sh::kTileBytes;
-                    for (int x = first * CH + i; x < kTile * CH; x += 128)   // zeros: the swizzle does not matter
-                        *reinterpret_cast<uint4*>(v + ((x % CH) >> 3) * (kTile * 128) + (x / CH) * 128 + (x & 7) * 16) =
-                            make_uint4(0u, 0u, 0u, 0u);
+                    for (int x = from * CH + i; x < kTile * CH; x += 128) {
+                        const int r = x / CH, ch = x % CH;
+                        uint4* at = reinterpret_cast<uint4*>(v + (ch >> 3) * (kTile * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
+                        uint4 y = make_uint4(0u, 0u, 0u, 0u);
+                        if (r < left) {
+                            y = *at;
+                            if (!mend_chunk(y)) continue;
+                            mended = true;
+                        }
+                        *at = y;
+                    }
+                    if (mended) s_mended = 1;
                     fence_async_smem();
                     named_bar_sync(1, 128);
                     if (i == 0) mbar_arrive(smem_u32(&bars.full[slot]));
@@ -419,6 +496,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
                             *reinterpret_cast<uint4*>(dst + k * RC * 128 + x0 * 16) = make_uint4(o[0], o[1], o[2], o[3]);
                             *reinterpret_cast<uint4*>(dst + k * RC * 128 + x1 * 16) = make_uint4(o[4], o[5], o[6], o[7]);
                         }
+                        if (kv == 1 && j >= first_masked && mend_rows<HD>(dst - row_at, i, max(0, all_see - (t0 + j) * kTile)))
+                            s_mended = 1;
                         fence_async_smem();
                         mbar_arrive(smem_u32(&bars.full[slot]));
                         mbar_arrive(smem_u32(&bars.raw_empty[st]));
@@ -600,30 +679,45 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
                 tc_wait(&bars.o_done, 0, &s_abort, fault);
                 tc_fence_after();
             }
+            const int from = max(all_see, t0 * kTile), to = min(limit, t1 * kTile);   // what this row sees of the masked
+            const bool mended = n > 0 && valid && s_mended != 0;
             if (S == 1) {
                 const float inv = l > 0.f ? 1.f / l : 0.f;
-                __half* dst = a.out + (long long)(seq.row0 + tok) * a.NH * HD + head * HD;
+                // this warp's 32 rows of the output, FP16, in Q's place (every product with Q is done), chunks xor row
+                constexpr int CH = HD / 8;
+                uint4* stage = reinterpret_cast<uint4*>(q_s) + (size_t)(i * kTile + (warp & 3) * 32) * CH;
 #pragma unroll
                 for (int h = 0; h < HD / 32; ++h) {
                     uint32_t o[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0u;
                     if (n > 0) {
                         tmem_ld(o_at + h * 32, o);
                         tmem_wait_ld();
                         tmem_pin(o);
                     }
-                    if (valid) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            uint32_t w[4];
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t w[4];
 #pragma unroll
-                            for (int x = 0; x < 4; ++x)
-                                w[x] = n > 0 ? pack_half2(__uint_as_float(o[8 * e + 2 * x]) * inv,
-                                                          __uint_as_float(o[8 * e + 2 * x + 1]) * inv)
-                                             : 0u;
-                            reinterpret_cast<uint4*>(dst + h * 32)[e] = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
+                        for (int x = 0; x < 4; ++x)
+                            w[x] = pack_half2(__uint_as_float(o[8 * e + 2 * x]) * inv, __uint_as_float(o[8 * e + 2 * x + 1]) * inv);
+                        stage[lane * CH + ((h * 4 + e) ^ (lane & 7))] = make_uint4(w[0], w[1], w[2], w[3]);
                     }
-                    __syncwarp();
+                }
+                __syncwarp();
+                const int first = row_base + i * kTile + (warp & 3) * 32, c = lane % CH;
+                const int count = min(32, rows - (i * kTile + (warp & 3) * 32));
+#pragma unroll 4
+                for (int x = lane / CH; x < count; x += 32 / CH) {
+                    const int t = (first + x) / a.G;
+                    __half* dst = a.out + ((long long)(seq.row0 + t) * a.NH + kvh * a.G + first + x - t * a.G) * HD;
+                    reinterpret_cast<uint4*>(dst)[c] = stage[x * CH + (c ^ (x & 7))];
+                }
+                __syncwarp();
+                if (mended) {
+                    add_mended<FMT, HD>(p, b, kvh, from, to, a.out + ((long long)(seq.row0 + tok) * a.NH + head) * HD, nullptr,
+                                        r, fault);
                 }
             } else {
                 // this CTA's part of the rows: 16-byte chunks
@@ -634,13 +728,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
 #pragma unroll
                 for (int h = 0; h < HD / 32; ++h) {
                     uint32_t o[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0u;
                     if (n > 0) {
                         tmem_ld(o_at + h * 32, o);
                         tmem_wait_ld();
                         tmem_pin(o);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = 0u;
                     }
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
@@ -648,6 +741,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
                             make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
                                         __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
                 }
+                if (mended) add_mended<FMT, HD>(p, b, kvh, from, to, nullptr, reinterpret_cast<float*>(part), r, fault);
             }
         }
     }
