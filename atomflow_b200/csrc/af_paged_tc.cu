@@ -212,6 +212,26 @@ __device__ __forceinline__ bool elect_one() {
     return r != 0;
 }
 
+// A row's token and head of the group, and those of every `by`-th row after it without a division each (Q's 32 rows per
+// thread took 6 us with one).
+struct RowOf {
+    int tok, head, G, d_tok, d_head;
+    __device__ __forceinline__ RowOf(int row, int g, int by) : G(g) {
+        tok = row / g;
+        head = row - tok * g;
+        d_tok = by / g;
+        d_head = by - d_tok * g;
+    }
+    __device__ __forceinline__ void step() {
+        tok += d_tok;
+        head += d_head;
+        if (head >= G) {
+            head -= G;
+            ++tok;
+        }
+    }
+};
+
 struct Bars {
     uint64_t full[8], empty[8];          // ring slots
     uint64_t raw_full[4], raw_empty[4];  // staging of codes; FP16: the V tiles with masked positions (three at most)
@@ -406,12 +426,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
             constexpr int RS = 128 / CH;             // rows between a thread's rows (a multiple of 8)
             const int c = i % CH, r0 = i / CH;
             const uint32_t at = smem_u32(q_s) + (c >> 3) * (kTile * 128) + r0 * 128 + (((c & 7) ^ (r0 & 7)) << 4);
+            RowOf row(row_base + r0, a.G, RS);
+            const __half* base = a.q + (long long)seq.row0 * a.q_stride + (long long)kvh * a.G * HD + c * 8;
 #pragma unroll 4
-            for (int k = 0; k < kItemRows / RS; ++k) {
-                const int r = r0 + k * RS;
-                const int R = row_base + r, tok = R / a.G, hd = R - tok * a.G;
-                const bool ok = r < rows;
-                const __half* src = a.q + (ok ? (long long)(seq.row0 + tok) * a.q_stride + (kvh * a.G + hd) * HD + c * 8 : 0);
+            for (int k = 0; k < kItemRows / RS; ++k, row.step()) {
+                const bool ok = r0 + k * RS < rows;
+                const __half* src = ok ? base + row.tok * a.q_stride + row.head * HD : a.q;
                 const int rt = k * RS;               // r0 < RS: the tile is that of k * RS
                 cp_async16_zfill(at + (rt >> 7) * Sh::kTileBytes + (rt & 127) * 128, src, ok ? 16u : 0u);
             }
@@ -708,12 +728,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
                 __syncwarp();
                 const int first = row_base + i * kTile + (warp & 3) * 32, c = lane % CH;
                 const int count = min(32, rows - (i * kTile + (warp & 3) * 32));
+                RowOf row(first + lane / CH, a.G, 32 / CH);
+                __half* base = a.out + ((long long)seq.row0 * a.NH + kvh * a.G) * HD + c * 8;
 #pragma unroll 4
-                for (int x = lane / CH; x < count; x += 32 / CH) {
-                    const int t = (first + x) / a.G;
-                    __half* dst = a.out + ((long long)(seq.row0 + t) * a.NH + kvh * a.G + first + x - t * a.G) * HD;
-                    reinterpret_cast<uint4*>(dst)[c] = stage[x * CH + (c ^ (x & 7))];
-                }
+                for (int x = lane / CH; x < count; x += 32 / CH, row.step())
+                    *reinterpret_cast<uint4*>(base + ((long long)row.tok * a.NH + row.head) * HD) = stage[x * CH + (c ^ (x & 7))];
                 __syncwarp();
                 if (mended) {
                     add_mended<FMT, HD>(p, b, kvh, from, to, a.out + ((long long)(seq.row0 + tok) * a.NH + head) * HD, nullptr,
