@@ -16,6 +16,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libatomflow_b200.so"
 CLI = PKG / "af_generate"        # the C++ greedy-decode driver on the C ABI
+EXT = PKG / "_torch_ops.so"      # the paged operators for torch tensors (needs torch's headers)
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-cudart", "shared"]
 
@@ -30,7 +31,7 @@ def headers():
 
 
 def up_to_date() -> bool:
-    if not LIB.exists() or not CLI.exists():
+    if not LIB.exists() or not CLI.exists() or not EXT.exists():
         return False
     t = LIB.stat().st_mtime
     return all(p.stat().st_mtime <= t for p in sources() + headers())
@@ -69,7 +70,32 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     if verbose:
         print(" ".join(cmd))
     subprocess.run(cmd, check=True, cwd=str(PKG))
+    build_ext(verbose)
     return LIB
+
+
+def build_ext(verbose: bool = False) -> None:
+    """The torch module over the C ABI; skipped where torch is not installed (the library itself does not need it)."""
+    import importlib.util
+    import sysconfig
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        return
+    import torch
+    root = Path(spec.origin).parent
+    cuda = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
+    tmp = EXT.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", str(ROOT / "include"), "-isystem", str(root / "include"),
+           "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"),
+           "-isystem", str(cuda / "include"), "-isystem", sysconfig.get_paths()["include"],
+           "-o", str(tmp), str(CSRC / "af_torch.cpp"), "-L", str(PKG), "-latomflow_b200",
+           "-L", str(root / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd))
+    subprocess.run(cmd, check=True, cwd=str(PKG))
+    os.replace(tmp, EXT)
 
 
 if __name__ == "__main__":
