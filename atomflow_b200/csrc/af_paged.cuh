@@ -144,6 +144,33 @@ __device__ __forceinline__ uint32_t kv_pack4(const float (&x)[4], float scale) {
     }
 }
 
+// ---- V at positions that some row of a tile does not see ----
+// Such a row's weight is zero, but zero times an infinity or NaN is NaN: both attention kernels put zeros in their
+// place in the tile, and add them back to the rows that do see them.
+// V's element as the attention sees it.
+template <int FMT, int HD>
+__device__ float v_value(const Paged& p, int b, int pos, int kvh, int d, unsigned* fault) {
+    const int page = paged_page(p, b, pos, fault);
+    if (page < 0) return 0.f;
+    const uint8_t* at = p.v + paged_at(p, page, pos, kvh, HD * KvFormat<FMT>::kBytes);
+    if constexpr (FMT == AF_KV_F16) return __half2float(reinterpret_cast<const __half*>(at)[d]);
+    const float s = __half2float(p.vs[paged_scale(p, page, pos, kvh)]);
+    if constexpr (FMT == AF_KV_INT8) return (float)reinterpret_cast<const int8_t*>(at)[d] * s;
+    return (float)reinterpret_cast<const __nv_fp8_e4m3*>(at)[d] * s;
+}
+// Puts zeros in the place of infinities and NaN in a pair of FP16 values; whether there were any.
+__device__ __forceinline__ bool mend_half2(uint32_t& v) {
+    const bool lo = (v & 0x7c00u) == 0x7c00u, hi = (v & 0x7c000000u) == 0x7c000000u;
+    if (lo) v &= 0xffff0000u;
+    if (hi) v &= 0x0000ffffu;
+    return lo | hi;
+}
+__device__ __forceinline__ bool mend_chunk(uint4& v) {
+    const bool a = mend_half2(v.x), b = mend_half2(v.y), c = mend_half2(v.z), d = mend_half2(v.w);
+    return a | b | c | d;
+}
+
+
 // ---- host side (af_paged.cu) ----
 af_status paged_args(const af_paged_kv* kv, const af_paged_batch* batch, Paged* out);
 // The attention of few rows (af_paged_few.cu): every sequence of at most 8 (rows_bound <= 8) or kFewRows rows (tokens x

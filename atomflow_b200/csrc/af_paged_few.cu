@@ -113,6 +113,21 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
     return v;
 }
+__device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+// E4M3's NaN codes -> 0; whether there were any.
+__device__ __forceinline__ bool mend_codes(uint4& v) {
+    uint32_t* w = &v.x;
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t nan = __vcmpeq4(w[i] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+        any |= nan != 0;
+        w[i] &= ~nan;
+    }
+    return any;
+}
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {
     uint32_t v;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
@@ -232,6 +247,7 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ float s_m[W][ROWS], s_l[W][ROWS];
     __shared__ float c_m[ROWS], c_l[ROWS];   // this CTA's, for the cluster
+    __shared__ int s_mended[W];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     int S = 1, rank = 0, b, kvh, t0, t1;
     PagedSeq seq;
@@ -419,6 +435,7 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[t][nt][e] = 0.f;
 
+    bool mended = false;                             // V had infinities or NaN where some row does not look
     float r = 1.f;                                   // V's scales are about 1 / r
     uint32_t stage = ring, to = ring + D * (2 * F::kHalf);
     const uint32_t ring_end = ring + F::kStages * (2 * F::kHalf);
@@ -484,7 +501,7 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
             k1 *= __shfl_sync(0xffffffffu, x, g + 8);
             v0 = __shfl_sync(0xffffffffu, x, 16 + g);
             v1 = __shfl_sync(0xffffffffu, x, 24 + g);
-            up = fmaxf(fabsf(v0), fabsf(v1)) * r > kRise;
+            up = (fabsf(v0) < 65520.f && fabsf(v0) * r > kRise) || (fabsf(v1) < 65520.f && fabsf(v1) * r > kRise);
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -493,7 +510,19 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
                 s[nt][e] *= k0;
                 s[nt][2 + e] *= k1;
             }
-        if (pos0 + KT > seen_by_all) {
+        const bool tail = pos0 + KT > seen_by_all;
+        if (tail) {
+            if constexpr (FMT != AF_KV_INT8) {   // V there: zeros for infinities and NaN
+                for (int x = max(0, seen_by_all - pos0) * F::kCh + lane; x < KT * F::kCh; x += 32) {
+                    const uint32_t at = vs + F::at(x / F::kCh, x % F::kCh, true);
+                    uint4 y = lds128(at);
+                    if (FMT == AF_KV_F16 ? mend_chunk(y) : mend_codes(y)) {
+                        mended = true;
+                        sts128(at, y);
+                    }
+                }
+                __syncwarp();
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -512,7 +541,8 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
         if (__any_sync(0xffffffffu, up)) {
             float q = 1.f;                           // r's change
             if constexpr (FMT != AF_KV_F16) {
-                float t = fminf(fmaxf(fabsf(v0), fabsf(v1)), 65504.f);
+                // (scales that are not finite do not move r: they would take the others' weights out of FP16's range)
+                float t = fmaxf(fabsf(v0) < 65520.f ? fabsf(v0) : 0.f, fabsf(v1) < 65520.f ? fabsf(v1) : 0.f);
 #pragma unroll
                 for (int x = 4; x < 32; x <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
                 if (t * r > kRise || (r == 1.f && t > 0.f)) {   // (an FP16 scale's exponent: 2^-24 .. 2^16)
@@ -553,6 +583,15 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
                     s[nt][2 * h + e] = FMT == AF_KV_F16 ? w : w * (h ? v1 : v0);
                 }
             }
+        if (FMT != AF_KV_F16 && tail) {   // a scale may be an infinity or NaN
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    if (pos0 + g >= lim[nt][e]) s[nt][e] = 0.f;
+                    if (pos0 + g + 8 >= lim[nt][e]) s[nt][2 + e] = 0.f;
+                }
+        }
         uint32_t pb[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -586,6 +625,10 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
         }
     }
     cp_async_wait<0>();
+    if constexpr (FMT != AF_KV_INT8) {
+        const int any = __any_sync(0xffffffffu, mended);
+        if (lane == 0) s_mended[warp] = any;
+    }
     __syncthreads();   // every ring is idle: the warps' parts go there, FP32 [warp][row][HD]
     float* part = reinterpret_cast<float*>(smem);
     static_assert((size_t)(W + 1) * ROWS * HD * 4 <= F::kSmem, "parts fit");
@@ -635,6 +678,23 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
             const float f = s_m[w][r] == -INFINITY ? 0.f : ex2(s_m[w][r] - M);
             L = fmaf(s_l[w][r], f, L);
             add(v, reinterpret_cast<const float4*>(part)[(w * ROWS + r) * (HD / 4) + ch], f);
+        }
+        if constexpr (FMT != AF_KV_INT8) {   // what was taken out of V, for the rows that see it
+            int any = 0;
+#pragma unroll
+            for (int w = 0; w < W; ++w) any |= s_mended[w];
+            const int to = any ? min(max(0, ctx + r / a.G + 1), t1 * KT) : 0;
+#pragma unroll 1
+            for (int pos = max(seen_by_all, t0 * KT); pos < to; ++pos) {
+                auto bad = [&](int e) {
+                    const float y = v_value<FMT, HD>(p, b, pos, kvh, ch * 4 + e, fault);
+                    return fabsf(y) < 65520.f ? 0.f : y;
+                };
+                v.x += bad(0);
+                v.y += bad(1);
+                v.z += bad(2);
+                v.w += bad(3);
+            }
         }
         if (WAVE && t1 - t0 < tiles) {   // a piece of an item: the one that begins it, or a later one
             const long long at = ((long long)2 * blockIdx.x + (t0 == 0 ? 1 : 0)) * ROWS + r;

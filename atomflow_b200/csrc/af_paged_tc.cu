@@ -250,17 +250,6 @@ __device__ __forceinline__ bool tc_wait(const uint64_t* bar, uint32_t parity, vo
     return false;
 }
 
-// V's element as the attention sees it.
-template <int FMT, int HD>
-__device__ float v_value(const Paged& p, int b, int pos, int kvh, int d, unsigned* fault) {
-    const int page = paged_page(p, b, pos, fault);
-    if (page < 0) return 0.f;
-    const uint8_t* at = p.v + paged_at(p, page, pos, kvh, HD * KvFormat<FMT>::kBytes);
-    if constexpr (FMT == AF_KV_F16) return __half2float(reinterpret_cast<const __half*>(at)[d]);
-    const float s = __half2float(p.vs[paged_scale(p, page, pos, kvh)]);
-    if constexpr (FMT == AF_KV_INT8) return (float)reinterpret_cast<const int8_t*>(at)[d] * s;
-    return (float)reinterpret_cast<const __nv_fp8_e4m3*>(at)[d] * s;
-}
 // Adds to a row's output (FP16, or FP32 in a cluster's part) what was taken out of V at positions [from, to).  Rare and
 // out of line: the row's outputs are read back.
 template <int FMT, int HD>
@@ -276,18 +265,6 @@ __device__ __noinline__ void add_mended(const Paged& p, int b, int kvh, int from
             else dst[d] = __float2half_rn(__half2float(dst[d]) + x);
         }
 }
-// Puts zeros in the place of infinities and NaN in a pair of FP16 values; whether there were any.
-__device__ __forceinline__ bool mend_half2(uint32_t& v) {
-    const bool lo = (v & 0x7c00u) == 0x7c00u, hi = (v & 0x7c000000u) == 0x7c000000u;
-    if (lo) v &= 0xffff0000u;
-    if (hi) v &= 0x0000ffffu;
-    return lo | hi;
-}
-__device__ __forceinline__ bool mend_chunk(uint4& v) {
-    const bool a = mend_half2(v.x), b = mend_half2(v.y), c = mend_half2(v.z), d = mend_half2(v.w);
-    return a | b | c | d;
-}
-
 // The same for the chunks of a tile of codes that thread i has just converted, in rows from `from` on.
 template <int HD>
 __device__ __noinline__ bool mend_rows(unsigned char* tile, int i, int from) {

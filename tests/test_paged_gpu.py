@@ -608,3 +608,57 @@ def test_a_prompt_in_chunks_then_tokens(fmt):
         assert ((v.float() - x).abs() <= step_v).all()
         check_attention(c, nh, q=q, max_q=max(ql), max_kv=200)
     assert faults() == 0
+
+
+def _with_bad_values(fmt, ql, where, ctx, nkv=2, hd=128, page=16, bad=(math.inf, -math.inf, math.nan)):
+    """A cache whose V holds infinities and NaN at some positions of the last chunk, and the same without them."""
+    n = ctx + ql
+    c, clean = Cache(fmt, [n], [ql], nkv, hd, page, seed=7), Cache(fmt, [n], [ql], nkv, hd, page, seed=7)
+    dims = torch.arange(0, hd, 37, device=DEV)
+    for i, pos in enumerate(where):
+        pg, slot = c.where(0, pos, 1)
+        x = bad[i % len(bad)]
+        if fmt == "f16":
+            c.v[pg, slot, :, dims] = x
+        elif fmt == "fp8":
+            c.v.view(torch.uint8)[pg, slot, :, dims] = 0x7f          # the format has no infinity
+        else:
+            c.vs[pg, slot] = x                                       # the whole vector
+        if fmt != "int8":
+            c.k[pg, slot] = torch.full_like(c.k[pg, slot].float(), math.nan).to(c.k.dtype)
+    return c, clean, dims
+
+
+@pytest.mark.parametrize("fmt", list(FMT))
+@pytest.mark.parametrize("ql,ctx,hd", [(4, 300, 128), (4, 0, 64), (3, 5000, 128), (40, 100, 128), (200, 0, 64), (130, 9000, 128)])
+def test_infinities_and_nan_reach_only_the_rows_that_see_them(fmt, ql, ctx, hd):
+    """K and V of a chunk's later tokens are not finite: the earlier tokens' outputs do not change by a bit, the later
+    ones' are not finite where V is not."""
+    from atomflow_b200 import ops
+    first = ctx + ql // 2
+    c, clean, dims = _with_bad_values(fmt, ql, [first, ctx + ql - 1], ctx, hd=hd)
+    q = torch.randn(ql, 4, hd, device=DEV, generator=torch.Generator(device=DEV).manual_seed(0)).half()
+    for kw in (dict(max_q=ql, max_kv=ctx + ql), dict(max_q=ql, max_kv=1)):
+        got = ops.paged_attention(q, *c.args, **c.scales, **kw)
+        ref = ops.paged_attention(q, *clean.args, **clean.scales, **kw)
+        assert torch.equal(got[:ql // 2], ref[:ql // 2]) and torch.isfinite(ref).all()
+        seen = got[ql // 2:].float()
+        assert not torch.isfinite(seen if fmt == "int8" else seen[:, :, dims]).any()
+        if fmt != "f16":
+            assert seen[:, :, dims].isnan().any()
+    assert faults() == 0
+
+
+def test_an_infinity_in_v_gives_an_infinity():
+    """Finite K: the rows that see +inf in V are +inf there, exact elsewhere, in both kernels."""
+    from atomflow_b200 import ops
+    for ql in (3, 100):
+        c = Cache("f16", [300], [ql], 1, 128, 16, seed=2)
+        q, good = check_attention(c, 2, max_q=ql, tail=0)
+        pg, slot = c.where(0, 300 - ql // 2, 1)
+        c.v[pg, slot, 0, 5] = math.inf
+        out = ops.paged_attention(q, *c.args, max_q=ql)
+        rows = ql - ql // 2
+        assert torch.equal(out[:rows], good[:rows])
+        assert (out[rows:, :, 5] == math.inf).all()
+        assert torch.isfinite(out[rows:, :, 6:]).all()
