@@ -27,8 +27,8 @@
 //     of the second product straight from TMEM.  The order PV(0, j), QK(0, j+1),
 //     PV(1, j), QK(1, j+1) keeps the tensor core on one row tile while the other
 //     is in its softmax.
-//   * Warps 0-3 and 4-7 are the softmax of row tile 0 and 1, one row per thread:
-//     no shuffles.  O is rescaled only when the row's maximum has grown by more
+//   * Warps 0-3 and 4-7 load Q and are the softmax of row tile 0 and 1, one row per
+//     thread: no shuffles.  O is rescaled only when the row's maximum has grown by more
 //     than a factor 2^8 since the last rescale (P then stays below 2^8, exact
 //     range in FP16; l and O are FP32), which ends after the first few tiles.
 //   * P is rounded to FP16 for the second product: its error, 2^-12 of each
@@ -236,7 +236,7 @@ struct Bars {
     uint64_t full[8], empty[8];          // ring slots
     uint64_t raw_full[4], raw_empty[4];  // staging of codes; FP16: the V tiles with masked positions (three at most)
     uint64_t s_full[2], p_full[2];       // per row tile
-    uint64_t q_full, o_done;
+    uint64_t q_full[2], o_done;
 };
 
 // Bounded wait: false once the limit has passed (the fault bit is set).
@@ -354,8 +354,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
             mbar_init(smem_u32(&bars.raw_full[i]), 1);
             mbar_init(smem_u32(&bars.raw_empty[i]), 128);
         }
-        mbar_init(smem_u32(&bars.q_full), 128);
         for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&bars.q_full[i]), 128);
             mbar_init(smem_u32(&bars.s_full[i]), 1);
             mbar_init(smem_u32(&bars.p_full[i]), 128);
         }
@@ -379,7 +379,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
     const int last_token = (row_base + rows - 1) / a.G;
     const int end = max(0, ctx + last_token + 1);    // positions any row sees
     const int tiles = (end + kTile - 1) / kTile;
-    const int t0 = (int)((long long)tiles * rank / S), t1 = (int)((long long)tiles * (rank + 1) / S);
+    const int shift = 31 - __clz(S);                 // S is a power of two, at most 8: no division, no overflow
+    const int t0 = (tiles * rank) >> shift, t1 = (tiles * (rank + 1)) >> shift;
     const int n = t1 - t0;
     // positions that every row sees; tiles from first_masked on hold others
     const int all_see = max(0, ctx + row_base / a.G + 1), first_masked = max(0, all_see / kTile - t0);
@@ -389,34 +390,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
     float* part_o = reinterpret_cast<float*>(smem);
     float* part_m = part_o + kItemRows * HD;
     float* part_l = part_m + kItemRows;
-    static_assert((kItemRows * HD + 2 * kItemRows) * 4 <= Sh::kSmem - 1024, "parts fit");
+    static_assert((kItemRows * HD + 3 * kItemRows) * 4 <= Sh::kSmem - 1024, "parts fit");   // and the merge's factors
 
     auto any_abort = [&] { return __any_sync(0xffffffffu, s_abort != 0) != 0; };   // the same for the whole warp
 
     if (warp >= kConvWarp) {
-        // ------------------------------------------------ Q, conversion, mending
+        // --------------------------------------------------- conversion, mending
         // registers are handed over once, here, and never taken back: 2 x 184 + 56 + 88 = 4 x 128
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         const int i = threadIdx.x - kConvWarp * 32;
         if (n > 0) {
             constexpr int CH = HD / 8;               // 16-byte FP16 chunks of a row
-            constexpr int RS = 128 / CH;             // rows between a thread's rows (a multiple of 8)
-            const int c = i % CH, r0 = i / CH;
-            const uint32_t at = smem_u32(q_s) + (c >> 3) * (kTile * 128) + r0 * 128 + (((c & 7) ^ (r0 & 7)) << 4);
-            RowOf row(row_base + r0, a.G, RS);
-            const __half* base = a.q + (long long)seq.row0 * a.q_stride + (long long)kvh * a.G * HD + c * 8;
-#pragma unroll 4
-            for (int k = 0; k < kItemRows / RS; ++k, row.step()) {
-                const bool ok = r0 + k * RS < rows;
-                const __half* src = ok ? base + row.tok * a.q_stride + row.head * HD : a.q;
-                const int rt = k * RS;               // r0 < RS: the tile is that of k * RS
-                cp_async16_zfill(at + (rt >> 7) * Sh::kTileBytes + (rt & 127) * 128, src, ok ? 16u : 0u);
-            }
-            cp_async_commit();
             if constexpr (!Sh::kQuant) {
-                cp_async_wait<0>();
-                fence_async_smem();
-                mbar_arrive(smem_u32(&bars.q_full));
                 // V tiles with masked positions come by way of these warps: zeros past the end and in the place of
                 // infinities and NaN
                 bool mended = false;
@@ -460,9 +445,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
                     }
                 };
                 fetch(0);
-                cp_async_wait<0>();
-                fence_async_smem();
-                mbar_arrive(smem_u32(&bars.q_full));
                 for (int j = 0; j < n; ++j) {
                     s_scale[j & 1][0][i] = sk;
                     s_scale[j & 1][1][i] = sv;
@@ -530,12 +512,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
                 tc_fence_after();
             };
             if (n > 0) {
-                tc_wait(&bars.q_full, 0, &s_abort, fault);
                 full(0);
-                if (!any_abort() && elect_one()) {
-                    for (int i = 0; i < n_sub; ++i) qk(i, 0);
-                    tc_commit(smem_u32(&bars.empty[0]));
+                for (int i = 0; i < n_sub; ++i) {
+                    tc_wait(&bars.q_full[i], 0, &s_abort, fault);
+                    tc_fence_after();
+                    if (!any_abort() && elect_one()) qk(i, 0);
+                    __syncwarp();
                 }
+                if (!any_abort() && elect_one()) tc_commit(smem_u32(&bars.empty[0]));
                 __syncwarp();
                 for (int j = 0; j < n; ++j) {
                     const int mv = 2 * j + 1, mk = 2 * j + 2;
@@ -600,6 +584,23 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
         // ------------------------------------------------------------- softmax
         asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
         const int i = warp >> 2, r = threadIdx.x & 127;   // row tile, row (= TMEM lane)
+        if (n > 0 && i < n_sub) {                         // Q: this row tile
+            constexpr int CH = HD / 8, RS = 128 / CH;     // 16-byte chunks of a row, rows between a thread's (a multiple of 8)
+            const int c = r % CH, r0 = r / CH;
+            const uint32_t at = smem_u32(q_s) + i * Sh::kTileBytes + (c >> 3) * (kTile * 128) + r0 * 128 + (((c & 7) ^ (r0 & 7)) << 4);
+            RowOf row(row_base + i * kTile + r0, a.G, RS);
+            const __half* base = a.q + (long long)seq.row0 * a.q_stride + (long long)kvh * a.G * HD + c * 8;
+#pragma unroll 4
+            for (int k = 0; k < kTile / RS; ++k, row.step()) {
+                const bool ok = i * kTile + r0 + k * RS < rows;
+                const __half* src = ok ? base + row.tok * a.q_stride + row.head * HD : a.q;
+                cp_async16_zfill(at + k * RS * 128, src, ok ? 16u : 0u);
+            }
+            cp_async_commit();
+            cp_async_wait<0>();
+            fence_async_smem();
+            mbar_arrive(smem_u32(&bars.q_full[i]));
+        }
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t s_at = tmem + i * kTile + lanes, o_at = tmem + 2 * kTile + i * kTile + lanes;
         const int R = row_base + i * kTile + r;
@@ -746,31 +747,62 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
     if (warp == kMmaWarp) tmem_dealloc(tmem, kTmemCols);
     if (S > 1) {
         cluster.sync();   // every CTA's part is there
-        // the softmax warps merge: they hold the registers
-        const int sub_rows = n_sub * kTile;
-        const int lo = sub_rows * rank / S, cnt = sub_rows * (rank + 1) / S - lo;
-        for (int x = threadIdx.x; warp < kMmaWarp && x < cnt * (HD / 4); x += kMmaWarp * 32) {
-            const int r = lo + x / (HD / 4), ch = x % (HD / 4);
-            if (r >= rows) break;
-            float M = -INFINITY;
-            for (int u = 0; u < S; ++u) M = fmaxf(M, cluster.map_shared_rank(part_m, u)[r]);
-            float l = 0.f;
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int u = 0; u < S; ++u) {   // rank order: the same bits every time
-                const float mu = cluster.map_shared_rank(part_m, u)[r];
-                if (mu == -INFINITY) continue;   // nothing seen there
-                const float f = ex2((mu - M) * a.c);
-                l = fmaf(cluster.map_shared_rank(part_l, u)[r], f, l);
-                const float4 q = reinterpret_cast<const float4*>(cluster.map_shared_rank(part_o, u))[(size_t)r * (HD / 4) + (ch ^ (r & (HD / 4 - 1)))];
-                o.x = fmaf(q.x, f, o.x);
-                o.y = fmaf(q.y, f, o.y);
-                o.z = fmaf(q.z, f, o.z);
-                o.w = fmaf(q.w, f, o.w);
+        // The softmax warps merge (they hold the registers) this CTA's share of the rows, in rank order: the same bits
+        // every time.  First every part's factor per row, then the sums, several loads from the other CTAs in flight.
+        const int sub_rows = n_sub * kTile, lo = sub_rows * rank / S, cnt = min(sub_rows * (rank + 1) / S, rows) - lo;
+        float* factor = part_l + kItemRows;   // [S][cnt]
+        if (warp < kMmaWarp) {
+            constexpr int kMerge = kMmaWarp * 32;
+            for (int x = threadIdx.x; x < cnt; x += kMerge) {
+                float mu[kMaxSplit], lu[kMaxSplit], M = -INFINITY, L = 0.f;
+#pragma unroll
+                for (int u = 0; u < kMaxSplit; ++u) {
+                    mu[u] = u < S ? cluster.map_shared_rank(part_m, u)[lo + x] : -INFINITY;
+                    lu[u] = u < S ? cluster.map_shared_rank(part_l, u)[lo + x] : 0.f;
+                }
+#pragma unroll
+                for (int u = 0; u < kMaxSplit; ++u) M = fmaxf(M, mu[u]);
+#pragma unroll
+                for (int u = 0; u < kMaxSplit; ++u) {
+                    mu[u] = mu[u] == -INFINITY ? 0.f : ex2((mu[u] - M) * a.c);   // 0: nothing seen there
+                    L = fmaf(lu[u], mu[u], L);
+                }
+                const float inv = L > 0.f ? 1.f / L : 0.f;
+#pragma unroll
+                for (int u = 0; u < kMaxSplit; ++u)
+                    if (u < S) factor[u * cnt + x] = mu[u] * inv;
             }
-            const float inv = l > 0.f ? 1.f / l : 0.f;
-            const int R = row_base + r, tok = R / a.G;
-            __half* dst = a.out + (long long)(seq.row0 + tok) * a.NH * HD + (kvh * a.G + R - tok * a.G) * HD + ch * 4;
-            *reinterpret_cast<uint2*>(dst) = make_uint2(pack_half2(o.x * inv, o.y * inv), pack_half2(o.z * inv, o.w * inv));
+            named_bar_sync(2, kMerge);
+            constexpr int CH = HD / 4, kBatch = 4;
+            for (int x0 = threadIdx.x; x0 < cnt * CH; x0 += kBatch * kMerge) {
+                float4 o[kBatch];
+#pragma unroll
+                for (int y = 0; y < kBatch; ++y) o[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+                for (int u = 0; u < S; ++u) {
+                    const float4* part = reinterpret_cast<const float4*>(cluster.map_shared_rank(part_o, u));
+#pragma unroll
+                    for (int y = 0; y < kBatch; ++y) {
+                        const int x = x0 + y * kMerge, r = x / CH, ch = x % CH;
+                        if (x >= cnt * CH) break;
+                        const float4 q = part[(size_t)(lo + r) * CH + (ch ^ ((lo + r) & (CH - 1)))];
+                        const float f = factor[u * cnt + r];
+                        o[y].x = fmaf(q.x, f, o[y].x);
+                        o[y].y = fmaf(q.y, f, o[y].y);
+                        o[y].z = fmaf(q.z, f, o[y].z);
+                        o[y].w = fmaf(q.w, f, o[y].w);
+                    }
+                }
+#pragma unroll
+                for (int y = 0; y < kBatch; ++y) {
+                    const int x = x0 + y * kMerge, r = x / CH, ch = x % CH;
+                    if (x >= cnt * CH) break;
+                    const int R = row_base + lo + r, tok = R / a.G;
+                    __half* dst =
+                        a.out + ((long long)(seq.row0 + tok) * a.NH + kvh * a.G + R - tok * a.G) * HD + ch * 4;
+                    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_half2(o[y].x, o[y].y), pack_half2(o[y].z, o[y].w));
+                }
+            }
         }
         cluster.sync();   // no CTA leaves while another reads its part
     }
@@ -866,11 +898,23 @@ cudaError_t paged_chunk_launch(int format, int head_dim, const Paged& p, const v
     const long long items = rows / kItemRows + seqs;
     const long long clusters = items * p.NKV;
     if (items == 0) return cudaSuccess;
-    const int sms = device_sm_count();
-    // split an item's positions while the GPU has idle SMs and each CTA keeps four tiles
+    // Split an item's positions over S CTAs where that shortens the whole: waves of CTAs x (tiles of each + what a CTA
+    // costs beside its tiles, about 3 tiles' time alone and 6 in a cluster that merges).  Clusters leave SMs out: of 148,
+    // cudaOccupancyMaxActiveClusters gives 148, 148, 132 and 120 to clusters of 1, 2, 4 and 8 such CTAs.
+    // (128 new tokens x 4 over 8192, 16 items: S = 8, 16 clusters for 15 places, 64 us; S = 4 37 us.)
     const long long full_items = std::max((rows + kItemRows - 1) / kItemRows, seqs) * p.NKV;
+    const int sms = std::max(8, device_sm_count()), tiles = std::max(1, (max_kv + kTile - 1) / kTile);
+    const int place[4] = {sms, sms / 2 * 2, sms * 33 / 148 * 4, sms * 15 / 148 * 8};
     int S = 1;
-    while (S < kMaxSplit && full_items * S * 2 <= sms && (long long)max_kv >= (long long)S * 2 * 4 * kTile) S *= 2;
+    double best = 1e300;
+    for (int i = 0; 1 << i <= kMaxSplit && (i == 0 || tiles >= 4 << i); ++i) {   // four tiles per CTA at least
+        const long long ctas = full_items << i, waves = (ctas + place[i] - 1) / place[i];
+        const double cost = (double)waves * ((double)tiles / (1 << i) + (i == 0 ? 3. : 6.));
+        if (cost < best) {
+            best = cost;
+            S = 1 << i;
+        }
+    }
     if (clusters * S > 0x7fffffffll) return cudaErrorInvalidConfiguration;
     auto go = [&](auto fmt) {
         return head_dim == 128 ? launch<decltype(fmt)::value, 128>(p, a, (unsigned)clusters, S, fault, st)
