@@ -407,10 +407,11 @@ extern "C" af_status af_paged_attention(const af_paged_kv* kv, const af_paged_ba
     if (fault == nullptr) return cuda_fail(e, "af_paged_attention");
     const AttnPlan x = attn_plan(p, n_heads, max_rows, max_kv);
     const cudaStream_t cs = static_cast<cudaStream_t>(stream);
-    if (x.few)
-        e = paged_few_launch(kv->format, kv->head_dim, p, q, q_stride, n_heads, scale, x.few_rows, !x.chunk, x.kv, out,
-                             workspace, workspace_bytes, fault, cs);
-    if (x.chunk && e == cudaSuccess)
+    // the long sequences first: the short ones' CTAs fill the SMs that their last wave leaves idle
+    if (x.chunk)
         e = paged_chunk_launch(kv->format, kv->head_dim, p, q, q_stride, n_heads, scale, x.skip_rows, x.kv, out, fault, cs);
+    if (x.few && e == cudaSuccess)
+        e = paged_few_launch(kv->format, kv->head_dim, p, q, q_stride, n_heads, scale, x.few_rows, x.chunk, x.kv, out,
+                             workspace, workspace_bytes, fault, cs);
     return e == cudaSuccess ? AF_OK : cuda_fail(e, "af_paged_attention");
 }

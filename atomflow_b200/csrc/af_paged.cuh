@@ -174,11 +174,12 @@ __device__ __forceinline__ bool mend_chunk(uint4& v) {
 // ---- host side (af_paged.cu) ----
 af_status paged_args(const af_paged_kv* kv, const af_paged_batch* batch, Paged* out);
 // The attention of few rows (af_paged_few.cu): every sequence of at most 8 (rows_bound <= 8) or kFewRows rows (tokens x
-// query heads per kv head).  alone: sequences of more rows are recorded as a fault, no other kernel takes them.
+// query heads per kv head).  behind: the tensor-core kernel was launched just before and takes the others; this one may
+// begin while it still runs (they touch different rows).  Else sequences of more rows are recorded as a fault.
 constexpr int kFewRows = 16;
 size_t paged_few_workspace(int format, int head_dim, const Paged& p, int rows_bound, int max_kv);
 cudaError_t paged_few_launch(int format, int head_dim, const Paged& p, const void* q, long long q_stride, int n_heads,
-                             float scale, int rows_bound, bool alone, int max_kv, void* out, void* workspace,
+                             float scale, int rows_bound, bool behind, int max_kv, void* out, void* workspace,
                              size_t workspace_bytes, unsigned* fault, cudaStream_t st);
 // The tensor-core attention (af_paged_tc.cu) over every sequence of more than
 // skip_rows rows (tokens x query heads per kv head).

@@ -92,6 +92,7 @@ struct FewArgs {
     int NH, G;
     float c;       // scale * log2(e)
     int alone;     // no other kernel takes the sequences of too many rows: record them
+    int behind;    // launched while another kernel of the call may still run: end after it
     // one wave: partial O [2 ctas][ROWS][HD], m and l [2 ctas][ROWS], and for each CTA the item that begins in it and
     // goes on in the next ones: {first row, kv head, pieces (0: no such item), rows}
     float4* part_o;
@@ -253,6 +254,11 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
     PagedSeq seq;
     long long u0 = 0, u1 = 0, first = 0, share = 1;   // one wave: this CTA's piece
     int even = 0;
+    // What follows in the stream waits for this grid alone, so the grid must not end before the kernel it was launched
+    // behind: its first CTA waits for that one (the others leave, their places are free for more).
+    auto leave = [&] {
+        if (a.behind && blockIdx.x == 0) pdl_wait();
+    };
     if constexpr (WAVE) {
         pdl_launch_dependents();             // every CTA is resident: the merge may line up behind them
         __shared__ FewPiece s_piece;
@@ -270,7 +276,10 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
         first = s_piece.first;
         share = s_piece.share;
         even = s_piece.even;
-        if (b < 0) return;
+        if (b < 0) {
+            leave();
+            return;
+        }
     } else {
         cg::cluster_group cluster = cg::this_cluster();
         S = (int)cluster.num_blocks();
@@ -282,6 +291,7 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
         const long long rows = (long long)seq.q * a.G;
         if (rows == 0 || rows > ROWS) {      // the whole cluster leaves
             if (rows > ROWS && a.alone && threadIdx.x == 0) atomicOr(fault, (unsigned)AF_FAULT_PAGED);
+            leave();
             return;
         }
     }
@@ -715,12 +725,18 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
             a.part_head[blockIdx.x] =
                 make_int4(seq.row0, kvh, even > 0 ? even : (int)((u0 + tiles - 1) / share) - (int)blockIdx.x + 1, rows);
         u0 += t1 - t0;
-        if (u0 >= u1) return;
+        if (u0 >= u1) {
+            leave();
+            return;
+        }
         if (u0 - first >= (long long)tiles * p.NKV) {   // on to the next sequence that is ours
             first += (long long)tiles * p.NKV;
             do ++b;
             while (b < p.n_seqs && few_tiles<ROWS>(p, a, b, fault) == 0);
-            if (b >= p.n_seqs) return;
+            if (b >= p.n_seqs) {
+                leave();
+                return;
+            }
         }
         __syncthreads();   // the parts have been read: the rings are free
     } else {
@@ -744,6 +760,7 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
             }
             cluster.sync();   // no CTA leaves while another reads its part
         }
+        leave();
         return;
     }
   }
@@ -854,12 +871,21 @@ cudaError_t launch_as(const Paged& p, const FewArgs& a, const FewPlan& x, unsign
     cfg.blockDim = dim3(F::kThreads);
     cfg.dynamicSmemBytes = F::kSmem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = x.S;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (!WAVE) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = x.S;
+        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    if (a.behind) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+    }
     cfg.attrs = attr;
-    cfg.numAttrs = WAVE ? 0 : 1;
+    cfg.numAttrs = n;
     e = cudaLaunchKernelEx(&cfg, kernel, p, a, fault);
     if (e != cudaSuccess || !WAVE) return e;
     return launch_pdl(paged_few_merge_kernel<HD, NT>, dim3(x.ctas), dim3(BIG ? kMergeThreads : 256), 0, st, a);
@@ -902,7 +928,7 @@ size_t paged_few_workspace(int format, int head_dim, const Paged& p, int rows_bo
 }
 
 cudaError_t paged_few_launch(int format, int head_dim, const Paged& p, const void* q, long long q_stride, int n_heads,
-                             float scale, int rows_bound, bool alone, int max_kv, void* out, void* workspace,
+                             float scale, int rows_bound, bool behind, int max_kv, void* out, void* workspace,
                              size_t workspace_bytes, unsigned* fault, cudaStream_t st) {
     FewArgs a{};
     a.q = static_cast<const __half*>(q);
@@ -911,7 +937,8 @@ cudaError_t paged_few_launch(int format, int head_dim, const Paged& p, const voi
     a.NH = n_heads;
     a.G = n_heads / p.NKV;
     a.c = scale * 1.4426950408889634f;
-    a.alone = alone ? 1 : 0;
+    a.alone = behind ? 0 : 1;
+    a.behind = behind ? 1 : 0;
     return dispatch(format, head_dim, rows_bound, [&](auto fmt, auto hd, auto nt) {
         return launch<decltype(fmt)::value, decltype(hd)::value, decltype(nt)::value>(p, a, max_kv, workspace,
                                                                                       workspace_bytes, fault, st);

@@ -307,6 +307,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
     const int S = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int cid = blockIdx.x / S, kvh = cid % p.NKV, item = cid / p.NKV;
 
+    pdl_launch_dependents();   // the kernel of the short sequences may begin as soon as every CTA of this one has
+
     // ------------------------------------------------ which work item is ours
     if (warp == 0) {
         int seen = 0, fb = -1, ft = 0;
