@@ -19,13 +19,15 @@ __device__ unsigned int g_paged_faults;
 namespace {
 
 // ---------------------------------------------------------------- write
-// One CTA per token.  HD / 8 lanes hold one head's vector, lane l the pairs
-// (4l + i, 4l + i + HD/2): RoPE's partner is in the same thread, and each load
-// and store of the lanes is one contiguous run.  Bound by DRAM: the qkv rows in,
-// q and the codes out.  The loads of a thread's vectors are issued before the
-// token's sequence is searched, so the search hides behind them.
+// A CTA takes a few tokens.  HD / 8 lanes hold one head's vector, lane l the pairs (4l + i, 4l + i + HD/2): RoPE's
+// partner is in the same thread, and each load and store of the lanes is one contiguous run.  Bound by DRAM: the qkv
+// rows in, q and the codes out.  A token's place is a chain of dependent loads (offsets, length, page): all of a CTA's
+// tokens look theirs up at once, one thread each, while the first vectors are on their way, and the vectors of the next
+// batch are loaded before those of this one are worked on.  (5 x up to 2047 tokens of 48 heads of 128, FP8, 189 MB:
+// with one token per CTA 45 us.)
 constexpr int kWriteThreads = 256;
-constexpr int kWriteBatch = 3;   // vectors of one thread in flight: 48 per CTA pass at HD 128
+constexpr int kWriteBatch = 3;    // vectors of one thread in flight: 48 per CTA at HD 128
+constexpr int kWriteTokens = 8;   // tokens of a CTA at most
 
 struct WriteArgs {
     const __half* qkv;
@@ -33,6 +35,7 @@ struct WriteArgs {
     const float *cos, *sin;  // [max_seq][HD / 2], or NULL: no rotation
     __half* q_out;
     int NH, max_seq;
+    int tokens;              // of a CTA
 };
 
 // The framework's rotation (rope.cu of the reference, its fast-math contraction):
@@ -46,50 +49,76 @@ template <int FMT, int HD>
 __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const Paged p, const WriteArgs a,
                                                                     unsigned* fault) {
     constexpr int L = HD / 8, GROUPS = kWriteThreads / L, HALF = HD / 2;
-    const int t = blockIdx.x, grp = threadIdx.x / L, l = threadIdx.x % L;
+    __shared__ int s_pos[kWriteTokens], s_page[kWriteTokens];   // page -1: nothing to do
+    const int t0 = blockIdx.x * a.tokens, nt = min(a.tokens, p.n_tokens - t0);
+    const int grp = threadIdx.x / L, l = threadIdx.x % L;
     const bool rotate = a.cos != nullptr;
     const int first = rotate ? 0 : a.NH, nvec = a.NH + 2 * p.NKV;   // without rotation q stays where it is
-    const __half* row = a.qkv + (long long)t * a.stride;
-    uint2 lo[kWriteBatch], hi[kWriteBatch];
-    auto load = [&](int v0) {
+    struct Batch {
+        uint2 lo[kWriteBatch], hi[kWriteBatch];
+    };
+    auto load = [&](Batch& x, int t, int v0) {
+        const __half* row = a.qkv + (long long)(t0 + t) * a.stride + 4 * l;
 #pragma unroll
         for (int i = 0; i < kWriteBatch; ++i) {
             const int v = v0 + i * GROUPS;
-            if (v < nvec) {
-                lo[i] = __ldg(reinterpret_cast<const uint2*>(row + (long long)v * HD + 4 * l));
-                hi[i] = __ldg(reinterpret_cast<const uint2*>(row + (long long)v * HD + HALF + 4 * l));
+            x.lo[i] = x.hi[i] = make_uint2(0u, 0u);
+            if (t < nt && v < nvec) {
+                x.lo[i] = __ldg(reinterpret_cast<const uint2*>(row + (long long)v * HD));
+                x.hi[i] = __ldg(reinterpret_cast<const uint2*>(row + (long long)v * HD + HALF));
             }
         }
     };
-    load(first + grp);
-    const int b = paged_find(p, t);
-    const PagedSeq s = paged_seq(p, b, fault);
-    const int pos = paged_pos_of(s, t);
-    if (pos < 0) return;   // no sequence's row, or before position 0
-    if (rotate && pos >= a.max_seq) {
-        if (threadIdx.x == 0) atomicOr(fault, (unsigned)AF_FAULT_POSITION);
-        return;
+    Batch next;
+    int t = 0, v0 = first + grp;
+    load(next, t, v0);
+    if (threadIdx.x < nt) {
+        const int b = paged_find(p, t0 + threadIdx.x);
+        const int pos = paged_pos_of(paged_seq(p, b, fault), t0 + threadIdx.x);
+        int page = -1;
+        if (pos >= 0) {   // else no sequence's row, or before position 0
+            if (rotate && pos >= a.max_seq) atomicOr(fault, (unsigned)AF_FAULT_POSITION);
+            else page = paged_page(p, b, pos, fault);
+        }
+        s_pos[threadIdx.x] = pos;
+        s_page[threadIdx.x] = page;
     }
-    const int page = paged_page(p, b, pos, fault);
-    if (page < 0) return;
+    __syncthreads();
     float4 c = make_float4(1.f, 1.f, 1.f, 1.f), sn = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (rotate) {
-        c = __ldg(reinterpret_cast<const float4*>(a.cos + (long long)pos * HALF) + l);
-        sn = __ldg(reinterpret_cast<const float4*>(a.sin + (long long)pos * HALF) + l);
-    }
-    const float ca[4] = {c.x, c.y, c.z, c.w}, sa[4] = {sn.x, sn.y, sn.z, sn.w};
-    for (int v0 = first + grp; v0 < nvec; v0 += kWriteBatch * GROUPS) {
-        if (v0 != first + grp) load(v0);
+    long long at = 0, scale_at = 0;   // of the token's first kv head
+    __half* q_row = nullptr;
+    for (bool new_token = true; t < nt;) {
+        const Batch now = next;
+        const int tt = t, vv = v0;
+        v0 += kWriteBatch * GROUPS;
+        if (v0 - grp >= nvec) {
+            v0 = first + grp;
+            ++t;
+        }
+        load(next, t, v0);
+        const int page = s_page[tt], pos = s_pos[tt];
+        const bool first_batch = new_token;
+        new_token = t != tt;
+        if (page < 0) continue;   // the same for the whole CTA
+        if (first_batch) {
+            at = paged_at(p, page, pos, 0, HD * KvFormat<FMT>::kBytes);
+            scale_at = paged_scale(p, page, pos, 0);
+            q_row = a.q_out + (long long)(t0 + tt) * a.NH * HD;
+        }
+        if (rotate && first_batch) {
+            c = __ldg(reinterpret_cast<const float4*>(a.cos + (long long)pos * HALF) + l);
+            sn = __ldg(reinterpret_cast<const float4*>(a.sin + (long long)pos * HALF) + l);
+        }
+        const float ca[4] = {c.x, c.y, c.z, c.w}, sa[4] = {sn.x, sn.y, sn.z, sn.w};
 #pragma unroll
         for (int i = 0; i < kWriteBatch; ++i) {
-            const int v = v0 + i * GROUPS;
+            const int v = vv + i * GROUPS;
             if (v - grp >= nvec) break;   // uniform over the warp: the shuffles below take every lane
-            const bool on = v < nvec;
-            if (!on) lo[i] = hi[i] = make_uint2(0u, 0u);
-            const bool is_v = v >= a.NH + p.NKV;
+            const bool on = v < nvec, is_v = v >= a.NH + p.NKV;
+            uint2 lo = now.lo[i], hi = now.hi[i];
             if (rotate && !is_v) {
-                __half2* pl = reinterpret_cast<__half2*>(&lo[i]);
-                __half2* ph = reinterpret_cast<__half2*>(&hi[i]);
+                __half2* pl = reinterpret_cast<__half2*>(&lo);
+                __half2* ph = reinterpret_cast<__half2*>(&hi);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const float2 x = __half22float2(pl[j]), y = __half22float2(ph[j]);
@@ -101,40 +130,32 @@ __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const Paged 
                 }
             }
             const int h = v - a.NH - (is_v ? p.NKV : 0);   // kv head; negative for q
-            uint8_t* dst = (is_v ? p.v : p.k) + (h < 0 ? 0 : paged_at(p, page, pos, h, HD * KvFormat<FMT>::kBytes));
+            uint8_t* dst = (is_v ? p.v : p.k) + at + h * (HD * KvFormat<FMT>::kBytes);   // (not used for q)
             if constexpr (FMT == AF_KV_F16) {
                 if (on) {
-                    __half* out = v < a.NH ? a.q_out + ((long long)t * a.NH + v) * HD : reinterpret_cast<__half*>(dst);
-                    *reinterpret_cast<uint2*>(out + 4 * l) = lo[i];
-                    *reinterpret_cast<uint2*>(out + HALF + 4 * l) = hi[i];
+                    __half* out = v < a.NH ? q_row + v * HD : reinterpret_cast<__half*>(dst);
+                    *reinterpret_cast<uint2*>(out + 4 * l) = lo;
+                    *reinterpret_cast<uint2*>(out + HALF + 4 * l) = hi;
                 }
             } else {
-                float x[4], y[4];
-                const __half2* pl = reinterpret_cast<const __half2*>(&lo[i]);
-                const __half2* ph = reinterpret_cast<const __half2*>(&hi[i]);
-                float amax = 0.f;
+                const __half2 x[2] = {*reinterpret_cast<const __half2*>(&lo.x), *reinterpret_cast<const __half2*>(&lo.y)};
+                const __half2 y[2] = {*reinterpret_cast<const __half2*>(&hi.x), *reinterpret_cast<const __half2*>(&hi.y)};
+                // (NaN does not count)
+                const __half2 m2 = __hmax2(__hmax2(__habs2(x[0]), __habs2(x[1])), __hmax2(__habs2(y[0]), __habs2(y[1])));
+                __half m1 = __hmax(__low2half(m2), __high2half(m2));
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const float2 u = __half22float2(pl[j]), w = __half22float2(ph[j]);
-                    x[2 * j] = u.x;
-                    x[2 * j + 1] = u.y;
-                    y[2 * j] = w.x;
-                    y[2 * j + 1] = w.y;
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) amax = fmaxf(amax, fmaxf(fabsf(x[j]), fabsf(y[j])));
-#pragma unroll
-                for (int o = L / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                for (int o = L / 2; o > 0; o >>= 1) m1 = __hmax(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+                const float amax = m1 == m1 ? __half2float(m1) : 0.f;
                 if (on && v < a.NH) {
-                    __half* out = a.q_out + ((long long)t * a.NH + v) * HD;
-                    *reinterpret_cast<uint2*>(out + 4 * l) = lo[i];
-                    *reinterpret_cast<uint2*>(out + HALF + 4 * l) = hi[i];
+                    __half* out = q_row + v * HD;
+                    *reinterpret_cast<uint2*>(out + 4 * l) = lo;
+                    *reinterpret_cast<uint2*>(out + HALF + 4 * l) = hi;
                 } else if (on) {
                     const __half sc = kv_scale<FMT>(amax);
-                    const float f = __half2float(sc);
-                    *reinterpret_cast<uint32_t*>(dst + 4 * l) = kv_pack4<FMT>(x, f);
-                    *reinterpret_cast<uint32_t*>(dst + HALF + 4 * l) = kv_pack4<FMT>(y, f);
-                    if (l == 0) (is_v ? p.vs : p.ks)[paged_scale(p, page, pos, h)] = sc;
+                    const float f = __half2float(sc), rcp = __frcp_rn(f);
+                    *reinterpret_cast<uint32_t*>(dst + 4 * l) = kv_pack4<FMT>(x, f, rcp);
+                    *reinterpret_cast<uint32_t*>(dst + HALF + 4 * l) = kv_pack4<FMT>(y, f, rcp);
+                    if (l == 0) (is_v ? p.vs : p.ks)[scale_at + h] = sc;
                 }
             }
         }
@@ -321,11 +342,14 @@ extern "C" af_status af_paged_kv_write(const af_paged_kv* kv, const af_paged_bat
     cudaError_t e;
     unsigned* fault = paged_fault_word(&e);
     if (fault == nullptr) return cuda_fail(e, "af_paged_kv_write");
+    // tokens of a CTA: one while that leaves SMs idle, more once there are several CTAs for each
+    const int tokens = std::max(1, std::min(kWriteTokens, p.n_tokens / (8 * std::max(1, device_sm_count()))));
     const WriteArgs a{static_cast<const __half*>(qkv), qkv_stride, cos_tab, sin_tab, static_cast<__half*>(q_out),
-                      n_heads, max_seq};
+                      n_heads, max_seq, tokens};
+    const unsigned grid = (unsigned)(((long long)p.n_tokens + tokens - 1) / tokens);
     paged_dispatch(kv, [&](auto fmt, auto hd) {
         paged_write_kernel<decltype(fmt)::value, decltype(hd)::value>
-            <<<p.n_tokens, kWriteThreads, 0, static_cast<cudaStream_t>(stream)>>>(p, a, fault);
+            <<<grid, kWriteThreads, 0, static_cast<cudaStream_t>(stream)>>>(p, a, fault);
     });
     e = cudaGetLastError();
     return e == cudaSuccess ? AF_OK : cuda_fail(e, "paged_write_kernel");

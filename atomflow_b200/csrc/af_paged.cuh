@@ -123,24 +123,36 @@ __device__ __forceinline__ __half kv_scale(float amax) {
     const __half s = __float2half_ru(__fdiv_rn(amax, KvFormat<FMT>::kCodeMax));
     return __hmin(s, __float2half_rn(KvFormat<FMT>::kScaleMax));
 }
-// Four values -> four codes: round to nearest even of x / scale, saturating.
+// Four values -> four codes: round to nearest even of x / scale, saturating.  x and the scale are FP16 values, and the
+// quotient matters only to a code's half step (9 bits at most): unless it is such a border itself it is 2^-20 away from
+// one, relatively, so x * rcp would do; and where it is one, the residual's correction makes it exact (rcp = 1 / scale
+// correctly rounded, q = x rcp (1 + 2^-23) at worst, and q + (x - q scale) rcp is then exact to 2^-46 before its
+// rounding).  Infinities count as the largest FP16 value; NaN stays (INT8: 0).
 template <int FMT>
-__device__ __forceinline__ uint32_t kv_pack4(const float (&x)[4], float scale) {
+__device__ __forceinline__ uint32_t kv_pack4(const __half2 (&h)[2], float scale, float rcp) {
+    const __half2 top = __float2half2_rn(65504.f);
     float y[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = __fdiv_rn(x[i], scale);
+    for (int i = 0; i < 2; ++i) {
+        const float2 x = __half22float2(__hmin2_nan(__hmax2_nan(h[i], __hneg2(top)), top));
+        const float q0 = x.x * rcp, q1 = x.y * rcp;
+        y[2 * i] = fmaf(fmaf(-q0, scale, x.x), rcp, q0);
+        y[2 * i + 1] = fmaf(fmaf(-q1, scale, x.y), rcp, q1);
+    }
     if constexpr (FMT == AF_KV_FP8_E4M3) {
         const uint32_t a = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
         const uint32_t b = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
-        return a | (b << 16);
+        // the correction of a quotient of -0 is +0: the sign comes from x
+        const uint32_t sign = __byte_perm(*reinterpret_cast<const uint32_t*>(&h[0]), *reinterpret_cast<const uint32_t*>(&h[1]), 0x7531);
+        return a | (b << 16) | (sign & 0x80808080u);
     } else {
-        uint32_t w = 0;
+        uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int c = __float2int_rn(fminf(fmaxf(y[i], -127.f), 127.f));
-            w |= (uint32_t)(y[i] == y[i] ? c & 0xff : 0) << (8 * i);
+        for (int i = 0; i < 4; ++i) {   // + 1.5 * 2^23 rounds to the nearest integer and leaves it in the low bits
+            const float c = y[i] == y[i] ? fminf(fmaxf(y[i], -127.f), 127.f) : 0.f;
+            w[i] = __float_as_uint(c + 12582912.f);
         }
-        return w;
+        return __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
     }
 }
 
