@@ -6,6 +6,7 @@
 // one page is a stretch of the same token-major rows [NKV * HD] that the
 // one-sequence cache has, so a contiguous cache is a pool whose table counts up.
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <type_traits>
 
@@ -19,15 +20,15 @@ __device__ unsigned int g_paged_faults;
 namespace {
 
 // ---------------------------------------------------------------- write
-// A CTA takes a few tokens.  HD / 8 lanes hold one head's vector, lane l the pairs (4l + i, 4l + i + HD/2): RoPE's
+// A CTA takes a few tokens.  HD / 16 lanes hold one head's vector, lane l the pairs (8l + i, 8l + i + HD/2): RoPE's
 // partner is in the same thread, and each load and store of the lanes is one contiguous run.  Bound by DRAM: the qkv
 // rows in, q and the codes out.  A token's place is a chain of dependent loads (offsets, length, page): all of a CTA's
 // tokens look theirs up at once, one thread each, while the first vectors are on their way, and the vectors of the next
 // batch are loaded before those of this one are worked on.  (5 x up to 2047 tokens of 48 heads of 128, FP8, 189 MB:
-// with one token per CTA 45 us.)
-constexpr int kWriteThreads = 256;
-constexpr int kWriteBatch = 3;    // vectors of one thread in flight: 48 per CTA at HD 128
-constexpr int kWriteTokens = 8;   // tokens of a CTA at most
+// 39.5 us, 4.8 TB/s; with one token per CTA 46, with 256 threads 42, with 8-byte loads 41.)
+constexpr int kWriteThreads = 128;
+constexpr int kWriteBatch = 2;    // vectors of one thread in flight: 32 per CTA at HD 128
+constexpr int kWriteTokens = 4;   // tokens of a CTA at most
 
 struct WriteArgs {
     const __half* qkv;
@@ -48,24 +49,24 @@ __device__ __forceinline__ void rope_pair(float x, float y, float c, float s, fl
 template <int FMT, int HD>
 __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const Paged p, const WriteArgs a,
                                                                     unsigned* fault) {
-    constexpr int L = HD / 8, GROUPS = kWriteThreads / L, HALF = HD / 2;
+    constexpr int L = HD / 16, GROUPS = kWriteThreads / L, HALF = HD / 2;
     __shared__ int s_pos[kWriteTokens], s_page[kWriteTokens];   // page -1: nothing to do
     const int t0 = blockIdx.x * a.tokens, nt = min(a.tokens, p.n_tokens - t0);
     const int grp = threadIdx.x / L, l = threadIdx.x % L;
     const bool rotate = a.cos != nullptr;
     const int first = rotate ? 0 : a.NH, nvec = a.NH + 2 * p.NKV;   // without rotation q stays where it is
     struct Batch {
-        uint2 lo[kWriteBatch], hi[kWriteBatch];
+        uint4 lo[kWriteBatch], hi[kWriteBatch];
     };
     auto load = [&](Batch& x, int t, int v0) {
-        const __half* row = a.qkv + (long long)(t0 + t) * a.stride + 4 * l;
+        const __half* row = a.qkv + (long long)(t0 + t) * a.stride + 8 * l;
 #pragma unroll
         for (int i = 0; i < kWriteBatch; ++i) {
             const int v = v0 + i * GROUPS;
-            x.lo[i] = x.hi[i] = make_uint2(0u, 0u);
+            x.lo[i] = x.hi[i] = make_uint4(0u, 0u, 0u, 0u);
             if (t < nt && v < nvec) {
-                x.lo[i] = __ldg(reinterpret_cast<const uint2*>(row + (long long)v * HD));
-                x.hi[i] = __ldg(reinterpret_cast<const uint2*>(row + (long long)v * HD + HALF));
+                x.lo[i] = __ldg(reinterpret_cast<const uint4*>(row + (long long)v * HD));
+                x.hi[i] = __ldg(reinterpret_cast<const uint4*>(row + (long long)v * HD + HALF));
             }
         }
     };
@@ -84,7 +85,9 @@ __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const Paged 
         s_page[threadIdx.x] = page;
     }
     __syncthreads();
-    float4 c = make_float4(1.f, 1.f, 1.f, 1.f), sn = make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 c[2], sn[2];
+    c[0] = c[1] = make_float4(1.f, 1.f, 1.f, 1.f);
+    sn[0] = sn[1] = make_float4(0.f, 0.f, 0.f, 0.f);
     long long at = 0, scale_at = 0;   // of the token's first kv head
     __half* q_row = nullptr;
     for (bool new_token = true; t < nt;) {
@@ -106,21 +109,25 @@ __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const Paged 
             q_row = a.q_out + (long long)(t0 + tt) * a.NH * HD;
         }
         if (rotate && first_batch) {
-            c = __ldg(reinterpret_cast<const float4*>(a.cos + (long long)pos * HALF) + l);
-            sn = __ldg(reinterpret_cast<const float4*>(a.sin + (long long)pos * HALF) + l);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                c[j] = __ldg(reinterpret_cast<const float4*>(a.cos + (long long)pos * HALF) + 2 * l + j);
+                sn[j] = __ldg(reinterpret_cast<const float4*>(a.sin + (long long)pos * HALF) + 2 * l + j);
+            }
         }
-        const float ca[4] = {c.x, c.y, c.z, c.w}, sa[4] = {sn.x, sn.y, sn.z, sn.w};
+        const float ca[8] = {c[0].x, c[0].y, c[0].z, c[0].w, c[1].x, c[1].y, c[1].z, c[1].w};
+        const float sa[8] = {sn[0].x, sn[0].y, sn[0].z, sn[0].w, sn[1].x, sn[1].y, sn[1].z, sn[1].w};
 #pragma unroll
         for (int i = 0; i < kWriteBatch; ++i) {
             const int v = vv + i * GROUPS;
             if (v - grp >= nvec) break;   // uniform over the warp: the shuffles below take every lane
             const bool on = v < nvec, is_v = v >= a.NH + p.NKV;
-            uint2 lo = now.lo[i], hi = now.hi[i];
+            uint4 lo = now.lo[i], hi = now.hi[i];
+            __half2* pl = reinterpret_cast<__half2*>(&lo);
+            __half2* ph = reinterpret_cast<__half2*>(&hi);
             if (rotate && !is_v) {
-                __half2* pl = reinterpret_cast<__half2*>(&lo);
-                __half2* ph = reinterpret_cast<__half2*>(&hi);
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
+                for (int j = 0; j < 4; ++j) {
                     const float2 x = __half22float2(pl[j]), y = __half22float2(ph[j]);
                     float2 r0, r1;
                     rope_pair(x.x, y.x, ca[2 * j], sa[2 * j], r0.x, r1.x);
@@ -134,27 +141,29 @@ __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const Paged 
             if constexpr (FMT == AF_KV_F16) {
                 if (on) {
                     __half* out = v < a.NH ? q_row + v * HD : reinterpret_cast<__half*>(dst);
-                    *reinterpret_cast<uint2*>(out + 4 * l) = lo;
-                    *reinterpret_cast<uint2*>(out + HALF + 4 * l) = hi;
+                    *reinterpret_cast<uint4*>(out + 8 * l) = lo;
+                    *reinterpret_cast<uint4*>(out + HALF + 8 * l) = hi;
                 }
             } else {
-                const __half2 x[2] = {*reinterpret_cast<const __half2*>(&lo.x), *reinterpret_cast<const __half2*>(&lo.y)};
-                const __half2 y[2] = {*reinterpret_cast<const __half2*>(&hi.x), *reinterpret_cast<const __half2*>(&hi.y)};
                 // (NaN does not count)
-                const __half2 m2 = __hmax2(__hmax2(__habs2(x[0]), __habs2(x[1])), __hmax2(__habs2(y[0]), __habs2(y[1])));
+                __half2 m2 = __hmax2(__habs2(pl[0]), __habs2(ph[0]));
+#pragma unroll
+                for (int j = 1; j < 4; ++j) m2 = __hmax2(m2, __hmax2(__habs2(pl[j]), __habs2(ph[j])));
                 __half m1 = __hmax(__low2half(m2), __high2half(m2));
 #pragma unroll
                 for (int o = L / 2; o > 0; o >>= 1) m1 = __hmax(m1, __shfl_xor_sync(0xffffffffu, m1, o));
                 const float amax = m1 == m1 ? __half2float(m1) : 0.f;
                 if (on && v < a.NH) {
                     __half* out = q_row + v * HD;
-                    *reinterpret_cast<uint2*>(out + 4 * l) = lo;
-                    *reinterpret_cast<uint2*>(out + HALF + 4 * l) = hi;
+                    *reinterpret_cast<uint4*>(out + 8 * l) = lo;
+                    *reinterpret_cast<uint4*>(out + HALF + 8 * l) = hi;
                 } else if (on) {
                     const __half sc = kv_scale<FMT>(amax);
                     const float f = __half2float(sc), rcp = __frcp_rn(f);
-                    *reinterpret_cast<uint32_t*>(dst + 4 * l) = kv_pack4<FMT>(x, f, rcp);
-                    *reinterpret_cast<uint32_t*>(dst + HALF + 4 * l) = kv_pack4<FMT>(y, f, rcp);
+                    *reinterpret_cast<uint2*>(dst + 8 * l) =
+                        make_uint2(kv_pack4<FMT>(pl[0], pl[1], f, rcp), kv_pack4<FMT>(pl[2], pl[3], f, rcp));
+                    *reinterpret_cast<uint2*>(dst + HALF + 8 * l) =
+                        make_uint2(kv_pack4<FMT>(ph[0], ph[1], f, rcp), kv_pack4<FMT>(ph[2], ph[3], f, rcp));
                     if (l == 0) (is_v ? p.vs : p.ks)[scale_at + h] = sc;
                 }
             }
@@ -242,17 +251,19 @@ __global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const Paged p,
 namespace af {
 
 unsigned* paged_fault_word(cudaError_t* err) {
-    static unsigned* word[kMaxDevices];   // benign race: every writer stores the same address
+    static std::atomic<unsigned*> word[kMaxDevices];
     int dev = 0;
     *err = cudaGetDevice(&dev);
     if (*err != cudaSuccess || dev < 0 || dev >= kMaxDevices) return nullptr;
-    if (word[dev] == nullptr) {
+    unsigned* w = word[dev].load(std::memory_order_acquire);
+    if (w == nullptr) {
         void* ptr = nullptr;
         *err = cudaGetSymbolAddress(&ptr, g_paged_faults);
         if (*err != cudaSuccess) return nullptr;
-        word[dev] = static_cast<unsigned*>(ptr);
+        w = static_cast<unsigned*>(ptr);
+        word[dev].store(w, std::memory_order_release);
     }
-    return word[dev];
+    return w;
 }
 
 unsigned paged_faults(bool clear, cudaError_t* err) {
@@ -313,6 +324,12 @@ af_status paged_args(const af_paged_kv* kv, const af_paged_batch* batch, Paged* 
     return AF_OK;
 }
 
+// Whether [a, a + n) and [b, b + m) share a byte.
+static bool overlap(const void* a, long long n, const void* b, long long m) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + (uintptr_t)m && y < x + (uintptr_t)n;
+}
+
 // Calls f<FMT, HD>() for the cache's format and head size (checked by paged_args).
 template <class F>
 static void paged_dispatch(const af_paged_kv* kv, F&& f) {
@@ -338,7 +355,11 @@ extern "C" af_status af_paged_kv_write(const af_paged_kv* kv, const af_paged_bat
     if (cos_tab != nullptr && (max_seq < 1 || !aligned(cos_tab, 16) || !aligned(sin_tab, 16))) return AF_ERR_INVALID;
     if (p.n_seqs == 0 || p.n_tokens == 0) return AF_OK;
     if (qkv == nullptr || !aligned(qkv, 16)) return AF_ERR_INVALID;
-    if (cos_tab != nullptr && n_heads > 0 && (q_out == nullptr || !aligned(q_out, 16))) return AF_ERR_INVALID;
+    const long long row = (long long)(n_heads + 2 * p.NKV) * kv->head_dim;
+    if (cos_tab != nullptr && n_heads > 0 &&
+        (q_out == nullptr || !aligned(q_out, 16) ||
+         overlap(q_out, 2LL * p.n_tokens * n_heads * kv->head_dim, qkv, 2 * ((p.n_tokens - 1) * qkv_stride + row))))
+        return AF_ERR_INVALID;
     cudaError_t e;
     unsigned* fault = paged_fault_word(&e);
     if (fault == nullptr) return cuda_fail(e, "af_paged_kv_write");
@@ -361,7 +382,10 @@ extern "C" af_status af_paged_kv_read(const af_paged_kv* kv, const af_paged_batc
     const af_status st = paged_args(kv, batch, &p);
     if (st != AF_OK) return st;
     if (p.n_seqs == 0 || p.n_tokens == 0) return AF_OK;
-    if (k_out == nullptr || v_out == nullptr || !aligned(k_out, 16) || !aligned(v_out, 16)) return AF_ERR_INVALID;
+    const long long bytes = 2LL * p.n_tokens * p.NKV * kv->head_dim;
+    if (k_out == nullptr || v_out == nullptr || !aligned(k_out, 16) || !aligned(v_out, 16) ||
+        overlap(k_out, bytes, v_out, bytes))
+        return AF_ERR_INVALID;
     cudaError_t e;
     unsigned* fault = paged_fault_word(&e);
     if (fault == nullptr) return cuda_fail(e, "af_paged_kv_read");
@@ -425,7 +449,10 @@ extern "C" af_status af_paged_attention(const af_paged_kv* kv, const af_paged_ba
     if (q_stride < (int64_t)n_heads * kv->head_dim || q_stride % 8 != 0) return AF_ERR_INVALID;
     if (!(scale > 0.f) || !std::isfinite(scale) || !aligned(workspace, 16)) return AF_ERR_INVALID;
     if (p.n_seqs == 0 || p.n_tokens == 0) return AF_OK;
-    if (q == nullptr || out == nullptr || !aligned(q, 16) || !aligned(out, 16)) return AF_ERR_INVALID;
+    const long long row = (long long)n_heads * kv->head_dim;
+    if (q == nullptr || out == nullptr || !aligned(q, 16) || !aligned(out, 16) ||
+        overlap(out, 2 * p.n_tokens * row, q, 2 * ((p.n_tokens - 1) * q_stride + row)))
+        return AF_ERR_INVALID;
     cudaError_t e;
     unsigned* fault = paged_fault_word(&e);
     if (fault == nullptr) return cuda_fail(e, "af_paged_attention");

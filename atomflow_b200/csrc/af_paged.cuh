@@ -129,7 +129,8 @@ __device__ __forceinline__ __half kv_scale(float amax) {
 // correctly rounded, q = x rcp (1 + 2^-23) at worst, and q + (x - q scale) rcp is then exact to 2^-46 before its
 // rounding).  Infinities count as the largest FP16 value; NaN stays (INT8: 0).
 template <int FMT>
-__device__ __forceinline__ uint32_t kv_pack4(const __half2 (&h)[2], float scale, float rcp) {
+__device__ __forceinline__ uint32_t kv_pack4(__half2 h0, __half2 h1, float scale, float rcp) {
+    const __half2 h[2] = {h0, h1};
     const __half2 top = __float2half2_rn(65504.f);
     float y[4];
 #pragma unroll

@@ -19,10 +19,10 @@ struct PagedSeq {
     bool bad;
 };
 // From the sequence's two row offsets and its length.  Rows outside [0, n_tokens),
-// decreasing offsets, a negative length or one beyond max_pages pages: a bad
-// sequence, without rows.
+// decreasing offsets, a negative length or one beyond max_pages pages or 2^30
+// (so that a position plus a tile fits in an int): a bad sequence, without rows.
 AF_HD PagedSeq paged_seq_of(int s, int e, int kv, int n_tokens, int max_pages, int page_shift) {
-    if (s < 0 || e < s || e > n_tokens || kv < 0 || (int64_t)kv > ((int64_t)max_pages << page_shift))
+    if (s < 0 || e < s || e > n_tokens || kv < 0 || kv > (1 << 30) || (int64_t)kv > ((int64_t)max_pages << page_shift))
         return {0, 0, 0, true};
     return {s, e - s, kv, false};
 }

@@ -10,6 +10,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -33,6 +34,11 @@ struct TypeError : std::runtime_error {
 struct PythonError : std::exception {};   // already set
 
 [[noreturn]] void bad(const char* what) { throw ValueError(what); }
+
+// These operators serve; a gradient asked for would be lost without a word.
+void no_gradient(const at::Tensor& t) {
+    if (t.requires_grad() && c10::GradMode::is_enabled()) bad("the paged operators have no gradient: detach the input, or call under torch.no_grad()");
+}
 
 const at::Tensor& tensor(PyObject* o, const char* name) {
     if (!THPVariable_Check(o)) throw TypeError(std::string(name) + " must be a tensor");
@@ -162,6 +168,7 @@ PyObject* paged_kv_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Tensor& qkv = tensor(a[0], "qkv");
         const at::Tensor *cos = optional(a[7], "cos"), *sin = optional(a[8], "sin"), *q_out = optional(a[11], "q_out");
         if (qkv.dim() != 2) bad("qkv must be [T, (n_heads + 2 n_kv_heads) * head_dim]");
+        no_gradient(qkv);
         const int64_t T = qkv.size(0), nh = integer(a[6]);
         Paged p = paged(T, tensor(a[1], "k_pages"), tensor(a[2], "v_pages"), tensor(a[3], "block_table"),
                         tensor(a[4], "kv_len"), tensor(a[5], "cu_rows"), optional(a[9], "k_scale"), optional(a[10], "v_scale"));
@@ -223,6 +230,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 12, [&]() -> PyObject* {
         const at::Tensor& q = tensor(a[0], "q");
         if (q.dim() != 3) bad("q must be [T, n_heads, head_dim]");
+        no_gradient(q);
         const int64_t T = q.size(0), nh = q.size(1);
         Paged p = paged(T, tensor(a[1], "k_pages"), tensor(a[2], "v_pages"), tensor(a[3], "block_table"),
                         tensor(a[4], "kv_len"), tensor(a[5], "cu_rows"), optional(a[7], "k_scale"), optional(a[8], "v_scale"));

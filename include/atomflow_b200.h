@@ -349,7 +349,7 @@ af_status af_gemv_chain_fast(const af_chain_op* ops, int n_ops, void* workspace,
  * it, read and attention give zeros.
  * What the arrays hold cannot lead outside the buffers: a sequence whose rows
  * leave [0, n_tokens), whose offsets decrease or whose kv_len exceeds its
- * table is skipped, a page outside [0, n_pages) is written nowhere and read as
+ * table (or 2^30) is skipped, a page outside [0, n_pages) is written nowhere and read as
  * zeros, and each sets AF_FAULT_PAGED (af_device_faults).
  *
  *   af_paged_kv_write   qkv FP16 [n_tokens] rows [NH*HD | NKV*HD | NKV*HD],
@@ -379,7 +379,8 @@ af_status af_gemv_chain_fast(const af_chain_op* ops, int n_ops, void* workspace,
  *                       bounds (0: none of use), long caches of few rows are cut
  *                       evenly over the whole GPU instead of over clusters.
  *                       Calls that share a workspace must not overlap.
- * q, out, qkv, q_out, k_out, v_out 16-byte aligned.  No allocation. */
+ * q, out, qkv, q_out, k_out, v_out 16-byte aligned; an output overlaps no input
+ * and no other output.  No allocation. */
 typedef enum af_kv_format {
     AF_KV_F16 = 0,
     AF_KV_FP8_E4M3 = 1,

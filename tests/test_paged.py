@@ -55,7 +55,8 @@ def test_sequences_outside_the_buffers_have_no_rows(index):
                 (0, 2 ** 31 - 1, 4, 10, 4, 4)]:
         assert _seq(index, *bad) == (0, 0, 0, 1), bad
     # a table as wide as an int can say: the product does not overflow
-    assert _seq(index, 0, 1, 2 ** 31 - 1, 1, 2 ** 31 - 1, 8) == (0, 1, 2 ** 31 - 1, 0)
+    assert _seq(index, 0, 1, 2 ** 30, 1, 2 ** 31 - 1, 8) == (0, 1, 2 ** 30, 0)
+    assert _seq(index, 0, 1, 2 ** 30 + 1, 1, 2 ** 31 - 1, 8) == (0, 0, 0, 1)
 
 
 def test_positions_of_rows(index):
@@ -134,17 +135,24 @@ def test_bad_rows_are_refused():
     from atomflow_b200._lib import lib
     L, R = lib(), ctypes.byref
     kv, b = _c()
+    far = 1 << 20
 
     def write(qkv=4096, stride=8 * 128, heads=4, cos=None, sin=None, max_seq=0, q=None):
         return L.af_paged_kv_write(R(kv), R(b), qkv, stride, heads, cos, sin, max_seq, q, None)
 
-    def attend(q=4096, stride=4 * 128, heads=4, scale=0.1, rows=0, kvb=0, out=4096, ws=None):
+    def attend(q=4096, stride=4 * 128, heads=4, scale=0.1, rows=0, kvb=0, out=1 << 20, ws=None):
         return L.af_paged_attention(R(kv), R(b), q, stride, heads, scale, rows, kvb, out, ws, 0, None)
 
     assert write(qkv=None) == write(qkv=4104) == write(stride=8 * 128 - 8) == write(stride=8 * 128 + 4) == 1
-    assert write(heads=-1) == write(cos=4096, q=4096, max_seq=8) == write(cos=4096, sin=4096, q=4096) == 1
+    assert write(heads=-1) == write(cos=4096, q=far, max_seq=8) == write(cos=4096, sin=4096, q=far) == 1
     assert write(cos=4096, sin=4096, max_seq=8) == 1                        # no q_out
-    assert write(cos=4104, sin=4096, max_seq=8, q=4096) == 1
+    assert write(cos=4104, sin=4096, max_seq=8, q=far) == 1
+    # outputs over inputs, or over each other
+    for q in (4096, 4096 + 2 * 8 * 128 - 16, 4096 - 2 * 4 * 128 + 16):
+        assert write(cos=4096, sin=4096, max_seq=8, q=q) == 1
+    for out in (4096, 4096 + 2 * 4 * 128 - 16, 4096 - 2 * 4 * 128 + 16):
+        assert attend(out=out) == 1
+    assert L.af_paged_kv_read(R(kv), R(b), 4096, 4096 + 2 * 2 * 128 - 16, None) == 1
     assert attend(q=None) == attend(out=None) == attend(q=4104) == attend(out=4104) == 1
     assert attend(stride=4 * 128 - 8) == attend(stride=4 * 128 + 4) == attend(heads=3) == attend(heads=0) == 1
     assert attend(rows=-1) == attend(kvb=-1) == attend(ws=4104) == 1
@@ -200,6 +208,26 @@ def test_ops_refuse_scales_that_do_not_fit_the_format():
             ops.paged_attention(q, **t8, **{**s8, **bad})
     with pytest.raises(ValueError, match="n_heads"):
         ops.paged_attention(q[0], **t8, **s8)
+
+
+def test_ops_refuse_what_needs_a_gradient():
+    from atomflow_b200 import ops
+    t, s, q = _t()
+    with pytest.raises(ValueError, match="no gradient"):
+        ops.paged_attention(q.requires_grad_(), **t, **s)
+    with pytest.raises(ValueError, match="no gradient"):
+        ops.paged_kv_write(torch.zeros(1, 1024, dtype=torch.float16, requires_grad=True), n_heads=4, **t, **s)
+
+
+def test_ops_refuse_what_is_no_tensor_or_number():
+    from atomflow_b200 import ops
+    t, s, q = _t()
+    with pytest.raises(TypeError, match="q must be a tensor"):
+        ops.paged_attention([1.0], **t, **s)
+    with pytest.raises(TypeError):
+        ops.paged_kv_read(**t, n_rows=1.5, **s)
+    with pytest.raises(TypeError, match="cos must be a tensor"):
+        ops.paged_kv_write(torch.zeros(1, 1024, dtype=torch.float16), n_heads=4, cos=3, sin=4, **t, **s)
 
 
 def test_structures_match_the_header():

@@ -662,3 +662,99 @@ def test_an_infinity_in_v_gives_an_infinity():
         assert torch.equal(out[:rows], good[:rows])
         assert (out[rows:, :, 5] == math.inf).all()
         assert torch.isfinite(out[rows:, :, 6:]).all()
+
+
+@pytest.mark.parametrize("fmt", ["f16", "int8"])
+def test_mixed_batch_in_a_graph(fmt):
+    """Both kernels of a mixed batch, overlapping, captured with the write and the read around them and replayed: as eager."""
+    from atomflow_b200 import ops
+    nh, nkv, hd = 8, 2, 128
+    kv, ql = [700, 300, 5000, 64, 900, 33], [200, 1, 1, 64, 1, 3]
+    cos, sin = rope_tables(5000, hd)
+    c = Cache(fmt, kv, ql, nkv, hd, 16)
+    qkv = qkv_rows(c.T, nh, nkv, hd, 5)
+
+    def step():
+        q = ops.paged_kv_write(qkv, *c.args, n_heads=nh, cos=cos, sin=sin, **c.scales)
+        o = ops.paged_attention(q, *c.args, max_q=200, max_kv=5000, **c.scales)
+        return (q, o) + tuple(ops.paged_kv_read(*c.args, c.T, **c.scales))
+
+    eager = [t.clone() for t in step()]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs = step()
+    for _ in range(3):
+        for t in outs:
+            t.fill_(5.0)
+        g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, eager)) and faults() == 0
+    check_attention(c, nh, q=eager[0], max_q=200, max_kv=5000)
+
+
+def test_many_sequences_and_heads():
+    """More sequences than a warp looks at in one step, more kv heads than a CTA has warps, both kernels."""
+    kv = [1 + (37 * i) % 120 for i in range(150)]
+    ql = [min(n, 30) if i % 11 == 0 else min(n, 1 + i % 3) for i, n in enumerate(kv)]
+    c = Cache("int8", kv, ql, 3, 64, 8)
+    check_attention(c, 6, max_q=30, max_kv=120)
+    c = Cache("f16", [40] * 70, [1] * 70, 20, 64, 16)
+    check_attention(c, 20, max_q=1)
+
+
+@pytest.mark.parametrize("nh,nkv", [(64, 1), (200, 1)])
+def test_large_groups(nh, nkv):
+    """One kv head for many query heads: a single token's rows are a chunk's."""
+    c = Cache("fp8", [300, 17], [1, 3], nkv, 128, 16)
+    check_attention(c, nh, max_q=3, max_kv=300)
+
+
+def test_without_a_workspace():
+    """The C entry point with no workspace, or too small a one, gives the same result within the tolerance."""
+    import ctypes
+
+    from atomflow_b200 import lib
+    from atomflow_b200._lib import PagedBatch, PagedKv
+    c = Cache("f16", [40000, 9000], [1, 1], 1, 128, 64)
+    q, want = check_attention(c, 4, max_q=1, max_kv=40000, tail=0)
+    kv = PagedKv(0, c.k.shape[0], 64, 1, 128, c.k.data_ptr(), c.v.data_ptr(), c.k.stride(0), None, None, 0)
+    b = PagedBatch(2, 2, c.table.shape[1], c.cu.data_ptr(), c.len_t.data_ptr(), c.table.data_ptr(), c.table.shape[1])
+    L, R = lib(), ctypes.byref
+    need = L.af_paged_attention_workspace_bytes(R(kv), R(b), 4, 1, 40000)
+    assert need > 0
+    ws = torch.full((need,), 0xff, dtype=torch.uint8, device=DEV)     # any contents
+    st = torch.cuda.current_stream().cuda_stream
+    outs = []
+    for ptr, n in ((None, 0), (ws.data_ptr(), need - 1), (ws.data_ptr(), need), (ws.data_ptr(), need)):
+        out = torch.zeros_like(q)
+        assert L.af_paged_attention(R(kv), R(b), q.data_ptr(), 4 * 128, 4, 128 ** -0.5, 1, 40000, out.data_ptr(), ptr, n, st) == 0
+        outs.append(out)
+    assert faults() == 0
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[2], outs[3]) and torch.equal(outs[2], want)
+    row = 0
+    for i in range(2):
+        ref, tol = attention_f64(c, q, 128 ** -0.5, i, row)
+        assert ((outs[0][row:row + 1].double() - ref).abs() <= tol).all()
+        row += 1
+
+
+def test_refusals_of_the_library_reach_python():
+    from atomflow_b200 import AtomflowError, ops
+    c = Cache("f16", [16], [1], 1, 64, 16)
+    q = torch.zeros(1, 2, 64, dtype=torch.float16, device=DEV)
+    with pytest.raises(AtomflowError, match="invalid"):
+        ops.paged_attention(q, *c.args, scale=-1.0)
+    with pytest.raises(AtomflowError, match="invalid"):
+        ops.paged_attention(q, *c.args, out=q)                        # the output over the input
+    big = torch.zeros(2, 16, 1, 96, dtype=torch.float16, device=DEV)
+    with pytest.raises(AtomflowError, match="unsupported"):
+        ops.paged_attention(torch.zeros(1, 2, 96, dtype=torch.float16, device=DEV), big, big, *c.args[2:])
+    with pytest.raises(ValueError, match="pages' device"):
+        ops.paged_attention(q.cpu(), *c.args)
+    with pytest.raises(ValueError, match="one CUDA device"):
+        ops.paged_attention(q, *c.args[:3], c.len_t.cpu(), c.cu)
+    assert ops.paged_attention(q[:0], *c.args).shape == (0, 2, 64)    # nothing to do
+    assert faults() == 0
