@@ -523,7 +523,7 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
         const bool tail = pos0 + KT > seen_by_all;
         if (tail) {
             if constexpr (FMT != AF_KV_INT8) {   // V there: zeros for infinities and NaN
-                for (int x = max(0, seen_by_all - pos0) * F::kCh + lane; x < KT * F::kCh; x += 32) {
+                for (int x = max(0, seen_by_all - pos0) * F::kCh + lane; x < min(KT, end - pos0) * F::kCh; x += 32) {
                     const uint32_t at = vs + F::at(x / F::kCh, x % F::kCh, true);
                     uint4 y = lds128(at);
                     if (FMT == AF_KV_F16 ? mend_chunk(y) : mend_codes(y)) {
