@@ -13,8 +13,12 @@
 //     64-dim panel) through the block table, into a ring of slots in the
 //     128-byte-swizzled layout that the MMA reads; a page outside the pool is a
 //     coordinate outside the tensor, which reads as zeros.  8-bit codes land in a
-//     staging ring, and warps 12-15 multiply them by their scales into FP16 slots
-//     (the values af_paged_kv_read returns).
+//     staging ring, and warps 12-15 turn them into FP16 slots exactly: K's codes as
+//     they are, V's times their scale's power of two.  The rest of the scales is
+//     applied in FP32 by the softmax, K's to the columns of S, V's (in [1, 2)) to P
+//     before its rounding: multiplied into the FP16 slots they cost a rounding
+//     of every element (relative error against 64 bits of a 4096-token FP8 prompt
+//     3.9e-4, 130 us; as it is 2.7e-4, 152 us; FP32 scales in shared memory 152 us).
 //   * V at positions that a row does not see (behind it in its own chunk, or past the
 //     end) meets weights of zero; where it is an infinity or NaN the product would be
 //     NaN.  Warps 12-15 put zeros in the place of such values, and the epilogue adds
@@ -68,6 +72,9 @@ struct Shape {
     static constexpr int kSlots = HD == 64 ? 8 : kQuant ? 4 : 5;
     static constexpr int kStages = kQuant ? (HD == 64 ? 4 : 2) : 0;
     static constexpr int kQBytes = 2 * kTileBytes;
+    // Scales of as many tiles: what writes tile j's has waited for the ring slot of V's tile j - 1, that is for the
+    // product with V's tile j - 1 - kSlots / 2, behind the softmax that read that tile's scales.
+    static constexpr int kScales = kQuant ? kSlots / 2 + 1 : 1;
     static constexpr int kRing = kQBytes, kStaging = kRing + kSlots * kTileBytes;
     static constexpr size_t kSmem = kStaging + (size_t)kStages * kCodeBytes + 1024;   // + alignment to 1 KB
     // the fetch ring: slots, or staging for codes
@@ -198,6 +205,25 @@ __device__ __forceinline__ void add2(float& a, float& b, float c, float d) {
     asm("add.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(y));
     asm("mov.b64 {%0,%1}, %2;" : "=f"(a), "=f"(b) : "l"(x));
 }
+// (a, b) * (c, d) of FP32 values in one packed product
+__device__ __forceinline__ void mul2(uint32_t& a, uint32_t& b, float c, float d) {
+    unsigned long long x, y;
+    asm("mov.b64 %0, {%1,%2};" : "=l"(x) : "r"(a), "r"(b));
+    asm("mov.b64 %0, {%1,%2};" : "=l"(y) : "f"(c), "f"(d));
+    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(y));
+    asm("mov.b64 {%0,%1}, %2;" : "=r"(a), "=r"(b) : "l"(x));
+}
+// Eight FP16 scales of shared memory (16-byte aligned) in FP32
+__device__ __forceinline__ void scales8(const __half* p, float (&f)[8]) {
+    const uint4 q = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        f[2 * i] = x.x;
+        f[2 * i + 1] = x.y;
+    }
+}
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -300,7 +326,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
     __shared__ volatile int s_abort;
     __shared__ volatile int s_mended;                // V had infinities or NaN where some row does not look
     __shared__ int s_item[2];                        // sequence, row tile pair
-    __shared__ __half s_scale[2][2][kTile];          // two tiles' scales: K's, V's
+    // tiles' scales: K's, and V's without its power of two
+    __shared__ __align__(16) __half s_scale[Sh::kScales][2][kTile];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     cg::cluster_group cluster = cg::this_cluster();
@@ -431,13 +458,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
             } else {
                 constexpr int C8 = HD / 16;          // 16-code chunks of a row
                 constexpr int RC = 128 / C8, KR = kTile / RC;
-                const int c8 = i % C8, q0 = i / C8;
+                const int c8 = i % C8, rq = i / C8;
                 // code chunk c8 makes FP16 chunks 2 c8 and 2 c8 + 1 of panel c8 / 4
-                const uint32_t row_at = (c8 >> 2) * (kTile * 128) + q0 * 128;
-                const uint32_t x0 = ((2 * c8) & 7) ^ (q0 & 7), x1 = ((2 * c8 + 1) & 7) ^ (q0 & 7);
-                __half sk, sv;                       // of position i of the next tile
+                const uint32_t row_at = (c8 >> 2) * (kTile * 128) + rq * 128;
+                const uint32_t x0 = ((2 * c8) & 7) ^ (rq & 7), x1 = ((2 * c8 + 1) & 7) ^ (rq & 7);
+                // a warp owns the rows that its threads convert: lane l row `mine`, row rq + x RC lane rq % RPW + RPW x
+                constexpr int RPW = 32 / C8;
+                const int mine = (i >> 5) * RPW + lane % RPW + RC * (lane / RPW);
+                __half sk, sv;                       // of row `mine` of the next tile
                 auto fetch = [&](int j) {
-                    const int pos = (t0 + j) * kTile + i;
+                    const int pos = (t0 + j) * kTile + mine;
                     sk = sv = __float2half_rn(0.f);
                     const int page = j < n && pos < end ? paged_page(p, b, pos, fault) : -1;
                     if (page >= 0) {
@@ -448,9 +478,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
                 };
                 fetch(0);
                 for (int j = 0; j < n; ++j) {
-                    s_scale[j & 1][0][i] = sk;
-                    s_scale[j & 1][1][i] = sv;
-                    named_bar_sync(1, 128);
+                    // V's scale = power * rest, both exact: rest in [1, 2), smaller for a subnormal scale
+                    const uint32_t bits = __half_as_ushort(sv);
+                    const bool tiny = (bits & 0x7c00u) == 0;
+                    const bool odd = (bits & 0x7c00u) == 0x7c00u;   // an infinity or NaN stays with the values, which are mended
+                    const uint32_t power = tiny ? 0x0400u : odd ? bits : bits & 0x7c00u;
+                    s_scale[j % Sh::kScales][0][mine] = sk;
+                    s_scale[j % Sh::kScales][1][mine] = tiny ? __hmul(sv, __float2half_rn(16384.f))
+                                                   : __ushort_as_half((unsigned short)(odd ? 0x3c00u : (bits & 0x83ffu) | 0x3c00u));
                     fetch(j + 1);
                     const int left = end - (t0 + j) * kTile;   // positions of the tile that exist
 #pragma unroll
@@ -462,17 +497,20 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
                         unsigned char* dst = ring + slot * Sh::kTileBytes + row_at;
 #pragma unroll
                         for (int k = 0; k < KR; ++k) {
-                            const int r = q0 + k * RC;
+                            const int r = rq + k * RC;
                             uint4 code = *reinterpret_cast<const uint4*>(src + k * 2048);
                             if (r >= left) code = make_uint4(0u, 0u, 0u, 0u);
-                            const __half2 s2 = __half2half2(s_scale[j & 1][kv][r]);
+                            const uint32_t pw = kv == 1 ? __shfl_sync(0xffffffffu, power, rq % RPW + RPW * k) * 0x10001u : 0u;
+                            const __half2 s2 = *reinterpret_cast<const __half2*>(&pw);
                             const uint32_t in[4] = {code.x, code.y, code.z, code.w};
                             uint32_t o[8];
 #pragma unroll
                             for (int w = 0; w < 4; ++w) {
                                 kv_unpack4<FMT>(in[w], o[2 * w], o[2 * w + 1]);
-                                o[2 * w] = mul_half2(o[2 * w], s2);
-                                o[2 * w + 1] = mul_half2(o[2 * w + 1], s2);
+                                if (kv == 1) {
+                                    o[2 * w] = mul_half2(o[2 * w], s2);
+                                    o[2 * w + 1] = mul_half2(o[2 * w + 1], s2);
+                                }
                             }
                             *reinterpret_cast<uint4*>(dst + k * RC * 128 + x0 * 16) = make_uint4(o[0], o[1], o[2], o[3]);
                             *reinterpret_cast<uint4*>(dst + k * RC * 128 + x1 * 16) = make_uint4(o[4], o[5], o[6], o[7]);
@@ -620,6 +658,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
                 tmem_wait_ld();
 #pragma unroll
                 for (int h = 0; h < 4; ++h) tmem_pin(v[h]);
+                const __half* sc = s_scale[j % Sh::kScales][0];
+                if constexpr (Sh::kQuant) {   // K's scales
+#pragma unroll
+                    for (int h = 0; h < kTile / 8; ++h) {
+                        float f[8];
+                        scales8(sc + 8 * h, f);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            mul2(v[h >> 2][(8 * h + 2 * e) & 31], v[h >> 2][(8 * h + 2 * e + 1) & 31], f[2 * e], f[2 * e + 1]);
+                    }
+                }
                 const int lim = limit - (t0 + j) * kTile;      // of this tile
                 if (__any_sync(0xffffffffu, lim < kTile)) {
 #pragma unroll
@@ -658,6 +707,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t w[32];
+                    float f[8];
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
                         float x = __uint_as_float(v[2 * h + (e >> 4)][(2 * e) & 31]);
@@ -666,7 +716,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
                         x = ex2(x);
                         y = ex2(y);
                         add2(l0, l1, x, y);
-                        w[e] = pack_half2(x, y);
+                        if constexpr (Sh::kQuant) {   // V's scales, without their powers of two
+                            if (e % 4 == 0) scales8(sc + kTile + h * 64 + 2 * e, f);
+                            uint32_t xb = __float_as_uint(x), yb = __float_as_uint(y);
+                            mul2(xb, yb, f[(2 * e) & 7], f[(2 * e + 1) & 7]);
+                            w[e] = pack_half2(__uint_as_float(xb), __uint_as_float(yb));
+                        } else {
+                            w[e] = pack_half2(x, y);
+                        }
                     }
                     tmem_st(s_at + h * 32, w);
                 }
@@ -903,7 +960,7 @@ cudaError_t paged_chunk_launch(int format, int head_dim, const Paged& p, const v
     // Split an item's positions over S CTAs where that shortens the whole: waves of CTAs x (tiles of each + what a CTA
     // costs beside its tiles, about 3 tiles' time alone and 6 in a cluster that merges).  Clusters leave SMs out: of 148,
     // cudaOccupancyMaxActiveClusters gives 148, 148, 132 and 120 to clusters of 1, 2, 4 and 8 such CTAs.
-    // (128 new tokens x 4 over 8192, 16 items: S = 8, 16 clusters for 15 places, 64 us; S = 4 37 us.)
+    // (128 new tokens x 4 over 8192, 16 items: S = 8, 16 clusters for 15 places, 64 us; S = 4 47 us.)
     const long long full_items = std::max((rows + kItemRows - 1) / kItemRows, seqs) * p.NKV;
     const int sms = std::max(8, device_sm_count()), tiles = std::max(1, (max_kv + kTile - 1) / kTile);
     const int place[4] = {sms, sms / 2 * 2, sms * 33 / 148 * 4, sms * 15 / 148 * 8};

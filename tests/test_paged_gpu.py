@@ -8,11 +8,10 @@ W = sum p_j |v_j| and w_j = exp(s_j - max s) the weights before the division:
   * P is rounded to FP16 before the product: 2^-11 W, and 2^-25 per weight that
     is subnormal in FP16, relative to a largest weight of at least 1:
     2^-25 sum |v_j| / sum w_j
-  * 8-bit caches: K and V are used as FP16 (code * scale, one rounding): 2^-11 W
-    for V; for K a score error of at most 2^-11 scale sum_d |q_d k_d|.  (The path
-    of few rows is more exact there: it scales S in FP32, and V's scale, brought
-    to about 1 for the largest, goes into the one rounding of P; a weight that is
-    then subnormal is off by 2^-25 of the largest scale's: 2^-25 n max|v| / sum w_j.)
+  * 8-bit caches: the codes are exact in FP16, K's scale multiplies S in FP32, and
+    V's goes into the one rounding of P (less a power of two, exact in FP16 with the
+    codes, or brought to about 1 for the largest; a weight that is then subnormal is
+    off by 2^-25 of the largest scale's: 2^-25 n max|v| / sum w_j)
   * scores, sums and products in FP32: a score error of 2^-24 (HD / 16 + 8) scale
     sum |q_d k_d| and of 2^-22 relative in each exponential's argument and
     value, and 2^-19 W for the sums (up to 2^4 partial orders, truncating
@@ -146,10 +145,8 @@ def attention_f64(c, q, scale, b, row):
     absqk = (x.abs() @ k.abs().transpose(1, 2) * scale).masked_fill(hidden, 0.0).amax(-1, keepdim=True) if n else top * 0
     d = absqk * (2.0 ** -24 * (hd / 16 + 8)) + 2.0 ** -22 * (s.masked_fill(hidden, 0.0).abs().amax(-1, keepdim=True) + 1 if n else 1)
     quant = c.fmt != "f16"
-    if quant:
-        d = d + 2.0 ** -11 * absqk
     seen = (~hidden).double()
-    tol = (2.0 ** -11 * out.abs() + 2.0 ** -25 + W * ((2 if quant else 1) * 2.0 ** -11 + torch.expm1(2 * d) + 2.0 ** -19) +
+    tol = (2.0 ** -11 * out.abs() + 2.0 ** -25 + W * (2.0 ** -11 + torch.expm1(2 * d) + 2.0 ** -19) +
            2.0 ** -25 * (seen @ v.abs()) / total.clamp(min=1e-300).clamp(min=1.0))
     if quant:
         tol = tol + 2.0 ** -25 * (seen @ v.abs().amax(-1, keepdim=True)) / total.clamp(min=1e-300).clamp(min=1.0)
@@ -662,6 +659,53 @@ def test_an_infinity_in_v_gives_an_infinity():
         assert torch.equal(out[:rows], good[:rows])
         assert (out[rows:, :, 5] == math.inf).all()
         assert torch.isfinite(out[rows:, :, 6:]).all()
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("ql", [3, 300])
+def test_scales_of_every_size(fmt, hd, ql):
+    """Neighbouring positions whose scales differ by powers of ten, down to subnormal ones, over many tiles."""
+    g = torch.Generator().manual_seed(hd + ql)
+    ctx = 2300
+    def values(low, high):
+        x = torch.randn(ctx, 2, hd, generator=g)
+        return x * 10.0 ** (torch.rand(ctx, 2, 1, generator=g) * (high - low) + low)
+    c = Cache(fmt, [ctx], [ql], 2, hd, 16, k=[values(-5, 0.3)], v=[values(-5, 3)])
+    assert (c.vs[c.where(0, 0, ctx)].float() < 2.0 ** -14).any()
+    check_attention(c, 4)
+    check_attention(c, 4, max_q=ql, max_kv=ctx)
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_scales_that_are_not_finite(fmt, hd, which, bad):
+    """Only the rows that see the position notice; the others are as with a scale of 1 there.  (K's scale multiplies
+    the score: an infinite one makes it +inf, the row NaN, or -inf, the weight zero.)"""
+    from atomflow_b200 import ops
+    ctx, at = 700, 600
+    for ql, first in ((300, 200), (16, 0), (2, 0)):   # from which row on it is seen
+        c = Cache(fmt, [ctx], [ql], 2, hd, 16)
+        pg, slot = (int(x) for x in c.where(0, at, 1))
+        scale = c.ks if which == "k" else c.vs
+        q = torch.randn(ql, 4, hd, generator=torch.Generator(device=DEV).manual_seed(2), device=DEV).half()
+        scale[pg, slot] = 1.0
+        want = ops.paged_attention(q, *c.args, **c.scales)
+        dot = torch.einsum("thd,hd->th", q.double(), c.values(0, at, 1)[0][0].repeat_interleave(2, 0))
+        scale[pg, slot] = bad
+        got = ops.paged_attention(q, *c.args, **c.scales)
+        assert faults() == 0
+        assert torch.equal(got[:first], want[:first])
+        got, dot = got[first:], dot[first:]
+        if math.isnan(bad):
+            assert got.isnan().all()
+        elif which == "v":
+            assert not got.isfinite().any()
+        else:
+            assert (dot.abs() > 2.0 ** -10).all()
+            assert got[dot > 0].isnan().all() and got[dot < 0].isfinite().all()
 
 
 @pytest.mark.parametrize("fmt", ["f16", "int8"])
