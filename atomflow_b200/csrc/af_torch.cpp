@@ -68,6 +68,8 @@ struct Paged {
 Paged paged(int64_t n_tokens, const at::Tensor& k, const at::Tensor& v, const at::Tensor& table, const at::Tensor& len,
             const at::Tensor& cu, const at::Tensor* ks, const at::Tensor* vs) {
     const char* one_device = "every tensor must be on one CUDA device";
+    for (const at::Tensor* t : {&k, &v, ks, vs})
+        if (t != nullptr) no_gradient(*t);
     Paged p{};
     const at::ScalarType type = k.scalar_type();
     if (type == at::kHalf) p.kv.format = AF_KV_F16;

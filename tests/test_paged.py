@@ -217,6 +217,12 @@ def test_ops_refuse_what_needs_a_gradient():
         ops.paged_attention(q.requires_grad_(), **t, **s)
     with pytest.raises(ValueError, match="no gradient"):
         ops.paged_kv_write(torch.zeros(1, 1024, dtype=torch.float16, requires_grad=True), n_heads=4, **t, **s)
+    for name in ("k_pages", "v_pages"):
+        bad = {**t, name: t[name].clone().requires_grad_()}
+        with pytest.raises(ValueError, match="no gradient"):
+            ops.paged_attention(q.detach(), **bad, **s)
+        with pytest.raises(ValueError, match="no gradient"):
+            ops.paged_kv_read(**bad, n_rows=1, **s)
 
 
 def test_ops_refuse_what_is_no_tensor_or_number():
