@@ -54,7 +54,8 @@ constexpr int kMergeThreads = 512;  // at most
 constexpr int KT = 16;             // positions of a tile
 constexpr int kLong = 2560;        // positions per CTA of a cluster past which the work is cut into one wave (16 FP16
                                    // sequences of 4096 over 8 heads: clusters of 2 44 us, wave 48; 4 FP8 of 32768:
-                                   // clusters of 8 71 us, wave 54)
+                                   // clusters of 8 71 us, wave 54; 48 ragged FP16 ones of up to 4099, 4 rows:
+                                   // clusters of 2 31 us, wave 33)
 constexpr float kRise = 16.f;      // V's scale times r past which r moves: P v_scale r <= 2^8 * 2^4
 constexpr float kGrow = 8.f;       // log2 of the growth of a score over the maximum that moves it
 
