@@ -26,8 +26,10 @@
 //   * 8-bit K goes from 16-byte words to A operands without a transpose: the
 //     MMA's k index is a sum, so its order is chosen as the bytes lie (Q is
 //     loaded in that order).  8-bit V pairs positions by byte permutes.
-//   * INT8 K is used as 1024 + code + 128, the byte as an FP16 mantissa; the
-//     accumulator starts at -1152 sum(q), which takes the offset out again.
+//   * INT8 codes are exact FP16 operands: the byte as a mantissa of 1024, less
+//     1152.  (Left in the operand and taken out of the accumulator as 1152 sum(q),
+//     the offset costs no instruction, but the accumulator then rounds at its
+//     size, up to 2^10 times the score's for a query that leans to one side.)
 //   * K's scale multiplies S in FP32.  V's goes into P: the weight P v_scale r is
 //     rounded to FP16 once, r a power of two that brings the scales met so far to
 //     about 1 (raised scales rescale O as a raised maximum does), and V's codes
@@ -153,13 +155,6 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
-}
-
-// Four INT8 codes -> 1152 + code as FP16 (two words).
-__device__ __forceinline__ void unpack4_offset(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    w ^= 0x80808080u;
-    lo = __byte_perm(w, 0x64646464u, 0x4140);
-    hi = __byte_perm(w, 0x64646464u, 0x4342);
 }
 
 // ---- one wave: every item's tiles in a row, sequence by sequence, head by head ----
@@ -411,28 +406,15 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
     }
     // the lane's rows of S^T and O^T: nt * 8 + 2c + e; each sees positions [0, lim)
     int lim[NT][2];
-    float m[NT][2], l[NT][2], s0[NT][2], o[MT][NT][4];
+    float m[NT][2], l[NT][2], o[MT][NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        float sum = 0.f;
-        if constexpr (FMT == AF_KV_INT8) {   // sum(q) of row nt * 8 + g, then of the lane's rows
-#pragma unroll
-            for (int s = 0; s < HD / 16; ++s)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&qf[s][nt][e]));
-                    sum += x.x + x.y;
-                }
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int r = nt * 8 + 2 * c + e;
             lim[nt][e] = r < rows ? max(0, ctx + r / a.G + 1) : 0;
             m[nt][e] = -INFINITY;
             l[nt][e] = 0.f;
-            s0[nt][e] = FMT == AF_KV_INT8 ? -1152.f * __shfl_sync(0xffffffffu, sum, (2 * c + e) * 4) : 0.f;
         }
     }
     const int seen_by_all = max(0, ctx + 1);         // positions that no row masks
@@ -473,7 +455,7 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[nt][e] = s0[nt][e & 1];
+            for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
         if constexpr (FMT == AF_KV_F16) {
 #pragma unroll
             for (int t = 0; t < HD / 16; ++t) {
@@ -491,13 +473,8 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
                     uint32_t a0, a1, a2, a3;
-                    if constexpr (FMT == AF_KV_INT8) {
-                        unpack4_offset(xw[t], a0, a2);
-                        unpack4_offset(yw[t], a1, a3);
-                    } else {
-                        kv_unpack4<FMT>(xw[t], a0, a2);
-                        kv_unpack4<FMT>(yw[t], a1, a3);
-                    }
+                    kv_unpack4<FMT>(xw[t], a0, a2);
+                    kv_unpack4<FMT>(yw[t], a1, a3);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
                         mma16816(s[nt], a0, a1, a2, a3, qf[4 * u + t][nt][0], qf[4 * u + t][nt][1]);
