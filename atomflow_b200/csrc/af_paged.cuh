@@ -113,6 +113,21 @@ __device__ __forceinline__ uint32_t mul_half2(uint32_t v, __half2 s) {
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// A scale = power * rest, exactly, power a power of two whose product with every code is an FP16 value (down to FP16's
+// subnormals: INT8's codes are whole numbers, E4M3's multiples of 2^-9) and at most 2^MAX.  rest is in [1, 2), below
+// that where the power is the smallest, above where it is the largest; a scale that is not finite is all rest.
+struct KvScaleParts {
+    __half power;
+    float rest;
+};
+template <int FMT, int MAX>
+__device__ __forceinline__ KvScaleParts kv_split_scale(float scale) {
+    constexpr int MIN = FMT == AF_KV_INT8 ? -24 : -15;
+    int e = (int)((__float_as_uint(scale) >> 23) & 255u) - 127;   // (an FP16 value is a normal FP32 one, or 0)
+    e = e > 15 ? 0 : min(max(e, MIN), MAX);
+    return {__float2half_rn(__uint_as_float((uint32_t)(e + 127) << 23)), scale * __uint_as_float((uint32_t)(127 - e) << 23)};
+}
+
 // The scale of a vector whose largest magnitude is amax: the smallest FP16 value
 // that brings it to at most the largest code (rounded up, so that no element
 // saturates however small the scale), 1 for a vector of zeros.  NaN elements do

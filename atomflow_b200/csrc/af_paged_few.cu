@@ -30,10 +30,12 @@
 //     1152.  (Left in the operand and taken out of the accumulator as 1152 sum(q),
 //     the offset costs no instruction, but the accumulator then rounds at its
 //     size, up to 2^10 times the score's for a query that leans to one side.)
-//   * K's scale multiplies S in FP32.  V's goes into P: the weight P v_scale r is
-//     rounded to FP16 once, r a power of two that brings the scales met so far to
-//     about 1 (raised scales rescale O as a raised maximum does), and V's codes
-//     are exact.  (Scaling V itself took 32 of 404 instructions per tile.)
+//   * K's scale multiplies S in FP32.  V's is split: its power of two into the
+//     codes' FP16 operands, exactly, the rest, in [1, 2), into P before its one
+//     rounding.  A position's weight so keeps its 11 bits whatever the scales
+//     around it are.  (With all of it in P, brought to about 1 by a power of two
+//     of the warp's, one vector of zeros, whose scale is 1, left the others'
+//     weights the bits of FP16's subnormals.)
 //   * Warps and CTAs merge in a fixed order: the same bits every time.
 //   * The loop is bound by issue slots as much as by DRAM: 8 warps per SM (two per
 //     scheduler) issued in 45% of the cycles and read the cache at 3.6 TB/s, so
@@ -58,8 +60,6 @@ constexpr int kLong = 2560;        // positions per CTA of a cluster past which 
                                    // sequences of 4096 over 8 heads: clusters of 2 44 us, wave 48; 4 FP8 of 32768:
                                    // clusters of 8 71 us, wave 54; 48 ragged FP16 ones of up to 4099, 4 rows:
                                    // clusters of 2 31 us, wave 33)
-constexpr float kRise = 16.f;      // V's scale times r past which r moves: P v_scale r <= 2^8 * 2^4
-constexpr float kGrow = 8.f;       // log2 of the growth of a score over the maximum that moves it
 
 // NT: 8-row column tiles; BIG: one CTA per SM with all its warps, else CTAs of four warps.
 template <int FMT, int HD, int NT, bool BIG>
@@ -76,6 +76,9 @@ struct Few {
     static constexpr int kRing = kPerSm == 4 ? 12 * 1024 : 16 * 1024;
     static constexpr int kStages = kRing / (2 * kHalf);
     static constexpr size_t kSmem = (size_t)W * kStages * 2 * kHalf;
+    // log2 of the growth of a score over the maximum that moves it: P times the rest of any finite scale stays finite
+    // in FP16 (2^7 * 511.75, 2^5 * 2047)
+    static constexpr float kGrow = FMT == AF_KV_F16 ? 8.f : FMT == AF_KV_FP8_E4M3 ? 7.f : 5.f;
     // Byte offset of chunk ch of row r in a tile.  The chunks of each 128-byte line are permuted so that the lanes
     // of one shared-memory access fall into different banks: FP16 rows are read by ldmatrix (8 rows, one chunk);
     // 8-bit K two rows by four chunks; 8-bit V four even (or odd) rows by 32 bytes.
@@ -155,6 +158,30 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
+}
+
+// The largest power of two of V's scale that goes into the codes: for INT8 the byte stands on 1152, whose product with
+// the power has to be an FP16 value.
+template <int FMT>
+constexpr int kPowerMax = FMT == AF_KV_INT8 ? 5 : 7;
+// Four codes times a pair of powers of two (even, odd bytes) -> four FP16 values, exactly.  INT8: the fused product takes
+// the 1152 off before the one rounding.
+template <int FMT>
+__device__ __forceinline__ void unpack4_scaled(uint32_t w, uint32_t power, uint32_t& lo, uint32_t& hi) {
+    const __half2 p = *reinterpret_cast<const __half2*>(&power);
+    if constexpr (FMT == AF_KV_INT8) {
+        w ^= 0x80808080u;
+        const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+        const __half2 off = __hmul2(p, __float2half2_rn(-1152.f));
+        const __half2 ra = __hfma2(*reinterpret_cast<const __half2*>(&a), p, off);
+        const __half2 rb = __hfma2(*reinterpret_cast<const __half2*>(&b), p, off);
+        lo = *reinterpret_cast<const uint32_t*>(&ra);
+        hi = *reinterpret_cast<const uint32_t*>(&rb);
+    } else {
+        kv_unpack4<FMT>(w, lo, hi);
+        lo = mul_half2(lo, p);
+        hi = mul_half2(hi, p);
+    }
 }
 
 // ---- one wave: every item's tiles in a row, sequence by sequence, head by head ----
@@ -430,7 +457,6 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
             for (int e = 0; e < 4; ++e) o[t][nt][e] = 0.f;
 
     bool mended = false;                             // V had infinities or NaN where some row does not look
-    float r = 1.f;                                   // V's scales are about 1 / r
     uint32_t stage = ring, to = ring + D * (2 * F::kHalf);
     const uint32_t ring_end = ring + F::kStages * (2 * F::kHalf);
     for (int j = 0; j < n; ++j) {
@@ -484,13 +510,18 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
         // scores in the exponent's base 2; positions a row does not see: -inf
         float k0 = a.c, k1 = a.c, v0 = 0.f, v1 = 0.f;
         bool up = false;
+        uint32_t pow0 = 0u, pow1 = 0u;               // V's powers of two at positions 2c, 2c + 1 and 2c + 8, 2c + 9
         if constexpr (FMT != AF_KV_F16) {
             const float x = __half2float(sc);
+            const KvScaleParts parts = kv_split_scale<FMT, kPowerMax<FMT>>(x);
             k0 *= __shfl_sync(0xffffffffu, x, g);
             k1 *= __shfl_sync(0xffffffffu, x, g + 8);
-            v0 = __shfl_sync(0xffffffffu, x, 16 + g);
-            v1 = __shfl_sync(0xffffffffu, x, 24 + g);
-            up = (fabsf(v0) < 65520.f && fabsf(v0) * r > kRise) || (fabsf(v1) < 65520.f && fabsf(v1) * r > kRise);
+            v0 = __shfl_sync(0xffffffffu, parts.rest, 16 + g);
+            v1 = __shfl_sync(0xffffffffu, parts.rest, 24 + g);
+            const uint32_t mine = __half_as_ushort(parts.power);
+            const uint32_t pair = __byte_perm(mine, __shfl_down_sync(0xffffffffu, mine, 1), 0x5410);
+            pow0 = __shfl_sync(0xffffffffu, pair, 16 + 2 * c);
+            pow1 = __shfl_sync(0xffffffffu, pair, 24 + 2 * c);
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -525,21 +556,9 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
 #pragma unroll
             for (int e = 0; e < 2; ++e) {   // (m = -inf: any score is above it, -inf is not)
                 const float t = fmaxf(s[nt][e], s[nt][2 + e]);
-                up |= t > m[nt][e] + kGrow;
+                up |= t > m[nt][e] + F::kGrow;
             }
         if (__any_sync(0xffffffffu, up)) {
-            float q = 1.f;                           // r's change
-            if constexpr (FMT != AF_KV_F16) {
-                // (scales that are not finite do not move r: they would take the others' weights out of FP16's range)
-                float t = fmaxf(fabsf(v0) < 65520.f ? fabsf(v0) : 0.f, fabsf(v1) < 65520.f ? fabsf(v1) : 0.f);
-#pragma unroll
-                for (int x = 4; x < 32; x <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
-                if (t * r > kRise || (r == 1.f && t > 0.f)) {   // (an FP16 scale's exponent: 2^-24 .. 2^16)
-                    const float to_one = __uint_as_float((254u << 23) - (__float_as_uint(t) & 0x7f800000u));
-                    q = to_one / r;
-                    r = to_one;
-                }
-            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -547,10 +566,9 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
                     float t = fmaxf(m[nt][e], fmaxf(s[nt][e], s[nt][2 + e]));
 #pragma unroll
                     for (int x = 4; x < 32; x <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
-                    float f = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - t);
+                    const float f = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - t);
                     m[nt][e] = t;
                     l[nt][e] *= f;
-                    f *= q;
 #pragma unroll
                     for (int x = 0; x < MT; ++x) {
                         o[x][nt][e] *= f;
@@ -558,8 +576,6 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
                     }
                 }
         }
-        v0 *= r;
-        v1 *= r;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -605,8 +621,8 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {   // dims 2h and 2h + 1 of the four
                     uint32_t a0, a1, a2, a3;
-                    kv_unpack4<FMT>(__byte_perm(w0, w1, h ? 0x7362 : 0x5140), a0, a1);
-                    kv_unpack4<FMT>(__byte_perm(w8, w9, h ? 0x7362 : 0x5140), a2, a3);
+                    unpack4_scaled<FMT>(__byte_perm(w0, w1, h ? 0x7362 : 0x5140), pow0, a0, a1);
+                    unpack4_scaled<FMT>(__byte_perm(w8, w9, h ? 0x7362 : 0x5140), pow1, a2, a3);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) mma16816(o[2 * d + h][nt], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
                 }
@@ -621,7 +637,6 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
     __syncthreads();   // every ring is idle: the warps' parts go there, FP32 [warp][row][HD]
     float* part = reinterpret_cast<float*>(smem);
     static_assert((size_t)(W + 1) * ROWS * HD * 4 <= F::kSmem, "parts fit");
-    const float back = 1.f / r;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -639,7 +654,7 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int d = FMT == AF_KV_F16 ? 16 * t2 + g + 8 * h : 32 * (t2 >> 1) + 4 * g + 2 * (t2 & 1) + h;
-                    part[(warp * ROWS + row) * HD + d] = o[t2][nt][2 * h + e] * back;
+                    part[(warp * ROWS + row) * HD + d] = o[t2][nt][2 * h + e];
                 }
         }
     __syncthreads();

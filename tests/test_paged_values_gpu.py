@@ -53,3 +53,58 @@ def test_queries_with_a_mean(fmt, hd, mean, std):
     q = (mean + std * torch.randn(7, 8, hd, generator=gen(3))).half().to(DEV)
     compare(c, q, max_q=4, max_kv=1000)
     compare(c, q, scale=0.02)
+
+
+# ---------------------------------------------------------------- V of very different sizes
+# P times the rest of V's scale is rounded to FP16: 2^-11 of itself, or, where it is subnormal, 2^-25, times a code and its
+# power of two: at most max|v_j|, and for E4M3 scales below the smallest power (2^-15) at most 448 2^-14 (either kernel).
+def tiny(c):
+    return 2.0 ** -25 * 448 * 2.0 ** -14 * max(c.kv_len) if c.fmt == "fp8" else 0.0
+
+
+def peaked(n, nkv, hd, top, seed):
+    """Keys whose position `top` scores 8 above the others, which differ a little, for queries with 8 in element 0."""
+    k = 0.3 * torch.randn(n, nkv, hd, generator=gen(seed))
+    k[..., 0] = 0.0
+    k[top, :, 0] = hd ** 0.5
+    return k
+
+
+def peaked_queries(ql, nh, hd, seed):
+    q = torch.randn(ql, nh, hd, generator=gen(seed))
+    q[..., 0] = 8.0
+    return q.half().to(DEV)
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("ql", [1, 4, 64])
+@pytest.mark.parametrize("std", [0.02, 0.005, 0.0005])
+@pytest.mark.parametrize("sink", [True, False])
+def test_zero_vectors_beside_small_values(fmt, hd, ql, std, sink):
+    """V of ordinary small values with vectors of zeros among them, whose scale is 1; the position with the largest weight
+    one of them, or not."""
+    n, nkv = 2048, 2
+    v = std * torch.randn(n, nkv, hd, generator=gen(4))
+    v[7::50] = 0.0
+    top = 57 if sink else 60
+    c = Cache(fmt, [n], [ql], nkv, hd, 16, k=[peaked(n, nkv, hd, top, 5)], v=[v])
+    assert (c.vs[c.where(0, 57, 1)] == 1).all() and (c.vs[c.where(0, 60, 1)] < 2.0 ** -10).all()
+    q = peaked_queries(ql, 8, hd, 6)
+    compare(c, q, extra=tiny(c), max_q=ql, max_kv=n)
+    compare(c, q, extra=tiny(c))
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("ql", [1, 64])
+def test_an_outlier_vector_in_v(fmt, hd, ql):
+    """One vector 2^12 times the others, at a score so low that it hardly counts: the others keep their bits."""
+    n, nkv = 1000, 2
+    v = 0.02 * torch.randn(n, nkv, hd, generator=gen(7))
+    v[3::64] *= 4096.0
+    k = peaked(n, nkv, hd, 500, 8)
+    k[3::64, :, 0] = -2 * hd ** 0.5
+    c = Cache(fmt, [n], [ql], nkv, hd, 16, k=[k], v=[v])
+    q = peaked_queries(ql, 8, hd, 9)
+    compare(c, q, extra=tiny(c), max_q=ql, max_kv=n)
