@@ -64,7 +64,6 @@ constexpr int kThreads = 512;
 constexpr int kMmaWarp = 8, kFetchWarp = 9, kConvWarp = 12;
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr int kMaxSplit = 8;
-constexpr float kGrow = 8.f;            // log2 of the growth of the maximum that forces a rescale
 constexpr int kTmemCols = 512;
 
 template <int FMT, int HD>
@@ -80,6 +79,11 @@ struct Shape {
     static constexpr int kScales = kQuant ? kSlots / 2 + 1 : 1;
     static constexpr int kRing = kQBytes, kStaging = kRing + kSlots * kTileBytes;
     static constexpr size_t kSmem = kStaging + (size_t)kStages * kCodeBytes + 1024;   // + alignment to 1 KB
+    // The largest power of two of V's scale in a slot (times the largest code, -128 among INT8's, a finite FP16 value),
+    // and log2 of the growth of the maximum that forces a rescale: P times the rest of any finite scale stays finite in
+    // FP16 (2^7 * 511.75, 2^8 * 255.9).
+    static constexpr int kPowerMax = FMT == AF_KV_INT8 ? 8 : 7;
+    static constexpr float kGrow = FMT == AF_KV_FP8_E4M3 ? 7.f : 8.f;
     // the fetch ring: slots, or staging for codes
     static constexpr int kFetch = kQuant ? kStages : kSlots;
 };
@@ -481,14 +485,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
                 };
                 fetch(0);
                 for (int j = 0; j < n; ++j) {
-                    // V's scale = power * rest, both exact: rest in [1, 2), smaller for a subnormal scale
-                    const uint32_t bits = __half_as_ushort(sv);
-                    const bool tiny = (bits & 0x7c00u) == 0;
-                    const bool odd = (bits & 0x7c00u) == 0x7c00u;   // an infinity or NaN stays with the values, which are mended
-                    const uint32_t power = tiny ? 0x0400u : odd ? bits : bits & 0x7c00u;
+                    // V's scale = power * rest, both exact; an infinity or NaN stays with the values, which are mended
+                    const KvScaleParts parts = kv_split_scale<FMT, Sh::kPowerMax>(__half2float(sv));
+                    const bool odd = (__half_as_ushort(sv) & 0x7c00u) == 0x7c00u;
+                    const uint32_t power = __half_as_ushort(odd ? sv : parts.power);
                     s_scale[j % Sh::kScales][0][mine] = sk;
-                    s_scale[j % Sh::kScales][1][mine] = tiny ? __hmul(sv, __float2half_rn(16384.f))
-                                                   : __ushort_as_half((unsigned short)(odd ? 0x3c00u : (bits & 0x83ffu) | 0x3c00u));
+                    s_scale[j % Sh::kScales][1][mine] = __float2half_rn(odd ? 1.f : parts.rest);
                     fetch(j + 1);
                     const int left = end - (t0 + j) * kTile;   // positions of the tile that exist
 #pragma unroll
@@ -687,7 +689,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
                     for (int h = 0; h < 4; ++h) mx[h] = fmaxf(mx[h], __uint_as_float(v[h][e]));
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                 // grow: the old sums are too large a scale off (or there is no scale yet)
-                const bool grow = top > m && !((top - m) * a.c <= kGrow);
+                const bool grow = top > m && !((top - m) * a.c <= Sh::kGrow);
                 if (__any_sync(0xffffffffu, grow)) {
                     const float f = grow ? (m == -INFINITY ? 0.f : ex2((m - top) * a.c)) : 1.f;
                     if (grow) m = top;

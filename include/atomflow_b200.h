@@ -367,7 +367,8 @@ af_status af_gemv_chain_fast(const af_chain_op* ops, int n_ops, void* workspace,
  *                       sequences; fewer rows: each sequence's last ones).
  *   af_paged_attention  out[row, h] = softmax(scale * q k^T) v over the
  *                       positions up to the row's own (8-bit formats: with
- *                       code * scale not rounded to FP16), q FP16 [n_tokens] rows
+ *                       code * scale not rounded to FP16, whatever finite scale a
+ *                       caller's own pool has), q FP16 [n_tokens] rows
  *                       [NH][HD] q_stride elements apart (a multiple of 8), out
  *                       FP16 [n_tokens][NH][HD], NH % NKV == 0.  max_rows and
  *                       max_kv are the host's bounds on a sequence's rows and

@@ -108,3 +108,33 @@ def test_an_outlier_vector_in_v(fmt, hd, ql):
     c = Cache(fmt, [n], [ql], nkv, hd, 16, k=[k], v=[v])
     q = peaked_queries(ql, 8, hd, 9)
     compare(c, q, extra=tiny(c), max_q=ql, max_kv=n)
+
+
+# ---------------------------------------------------------------- scales above those that the write stores
+def large_scales(fmt, ql, hd, n=1000, nkv=2):
+    """A pool filled by the caller: V's scales up to FP16's largest, values beyond FP16 that average out."""
+    c = Cache(fmt, [n], [ql], nkv, hd, 16, k=[0.1 * torch.randn(n, nkv, hd, generator=gen(10))])
+    at = c.where(0, 0, n)
+    e = torch.rand(n, nkv, generator=gen(11)) * 7 + 9                       # 2^9 .. 2^16
+    c.vs[at] = (2.0 ** e).clamp(max=65504.0).half().to(DEV)
+    c.vs[c.where(0, 500, 1)] = 65504.0
+    if fmt == "int8":
+        c.v[c.where(0, 17, 1)] = -128
+    return c
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("ql", [1, 4, 64])
+def test_scales_above_the_stored_ones(fmt, hd, ql):
+    """code * scale is not rounded to FP16: both kernels give the average, or an infinity where it is none of FP16."""
+    from atomflow_b200 import ops
+    c = large_scales(fmt, ql, hd)
+    q = torch.randn(ql, 8, hd, generator=gen(12)).half().to(DEV)
+    got = ops.paged_attention(q, *c.args, max_q=ql, max_kv=1000, **c.scales).double()
+    want, tol = attention_f64(c, q, hd ** -0.5, 0, 0)
+    assert faults() == 0 and not got.isnan().any()
+    inside = want.abs() + tol < 65504
+    assert inside.double().mean() > 0.05 and float(((got - want).abs() / tol)[inside].max()) <= 1
+    outside = want.abs() - tol > 65520
+    assert got[outside].isinf().all() and (got.sign() == want.sign())[outside].all()
