@@ -692,7 +692,7 @@ __global__ void __launch_bounds__(Few<FMT, HD, NT, BIG>::kThreads, Few<FMT, HD, 
             for (int pos = max(seen_by_all, t0 * KT); pos < to; ++pos) {
                 auto bad = [&](int e) {
                     const float y = v_value<FMT, HD>(p, b, pos, kvh, ch * 4 + e, fault);
-                    return fabsf(y) < 65520.f ? 0.f : y;
+                    return fabsf(y) < INFINITY ? 0.f : y;
                 };
                 v.x += bad(0);
                 v.y += bad(1);

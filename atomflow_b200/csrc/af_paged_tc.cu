@@ -293,7 +293,7 @@ __device__ __noinline__ void add_mended(const Paged& p, int b, int kvh, int from
 #pragma unroll 1
         for (int d = 0; d < HD; ++d) {
             const float x = v_value<FMT, HD>(p, b, pos, kvh, d, fault);
-            if (fabsf(x) < 65520.f) continue;
+            if (fabsf(x) < INFINITY) continue;
             if (part != nullptr) part[((d >> 2) ^ (r & (HD / 4 - 1))) * 4 + (d & 3)] += x;
             else dst[d] = __float2half_rn(__half2float(dst[d]) + x);
         }

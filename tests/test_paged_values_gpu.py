@@ -138,3 +138,21 @@ def test_scales_above_the_stored_ones(fmt, hd, ql):
     assert inside.double().mean() > 0.05 and float(((got - want).abs() / tol)[inside].max()) <= 1
     outside = want.abs() - tol > 65520
     assert got[outside].isinf().all() and (got.sign() == want.sign())[outside].all()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("ql", [4, 64])
+def test_nan_beside_values_beyond_fp16(hd, ql):
+    """What is put back for the rows that see a NaN is the NaN alone, not finite values that are none of FP16."""
+    from atomflow_b200 import ops
+    c = large_scales("fp8", ql, hd)
+    q = torch.randn(ql, 8, hd, generator=gen(13)).half().to(DEV)
+    c.vs[c.where(0, 0, 1000)] = 1.0
+    at = c.where(0, 1000 - ql // 2, ql // 2)                                # the last positions, masked for the first rows
+    c.vs[at] = 1024.0
+    c.v[at] = torch.full((ql // 2, 2, hd), 448.0, device=DEV).to(torch.float8_e4m3fn)
+    clean = ops.paged_attention(q, *c.args, max_q=ql, max_kv=1000, **c.scales)
+    c.v.view(torch.uint8)[c.where(0, 999, 1) + (slice(None), 3)] = 0x7f
+    got = ops.paged_attention(q, *c.args, max_q=ql, max_kv=1000, **c.scales)
+    assert faults() == 0 and torch.equal(got[:-1], clean[:-1]) and got[-1, :, 3].isnan().all()
+    assert torch.equal(got[-1, :, :3], clean[-1, :, :3]) and torch.equal(got[-1, :, 4:], clean[-1, :, 4:])
