@@ -45,4 +45,28 @@ AF_HD int64_t paged_scale_at(int page, int64_t scale_stride, int slot, int nkv, 
     return (int64_t)page * scale_stride + (int64_t)slot * nkv + head;
 }
 
+
+// Over how many CTAs (a power of two) the chunk kernel splits the positions of its work items, of at most `tiles` tiles
+// each, on a GPU of `sms` SMs (0 or less: not known): as many as shorten the whole, waves of CTAs x (tiles of each + what a
+// CTA costs beside its tiles, about 3 tiles' time alone and 6 in a cluster that merges).  Clusters leave SMs out: of 148,
+// cudaOccupancyMaxActiveClusters gives 148, 148, 132 and 120 to clusters of 1, 2, 4 and 8 such CTAs; a GPU too small for
+// a size does not use it.  (128 new tokens x 4 over 8192, 16 items: 8 CTAs, 16 clusters for 15 places, 64 us; 4 CTAs 47 us.)
+constexpr int kPagedMaxSplit = 8;
+inline int paged_chunk_split(int64_t items, int tiles, int sms) {
+    if (sms < 1) sms = 1;
+    const int place[4] = {sms, sms / 2 * 2, sms * 33 / 148 * 4, sms * 15 / 148 * 8};
+    int split = 1;
+    double best = 1e300;
+    for (int i = 0; 1 << i <= kPagedMaxSplit && (i == 0 || tiles >= 4 << i); ++i) {   // four tiles per CTA at least
+        if (place[i] == 0) continue;
+        const int64_t ctas = items << i, waves = (ctas + place[i] - 1) / place[i];
+        const double cost = (double)waves * ((double)tiles / (1 << i) + (i == 0 ? 3. : 6.));
+        if (cost < best) {
+            best = cost;
+            split = 1 << i;
+        }
+    }
+    return split;
+}
+
 }  // namespace af

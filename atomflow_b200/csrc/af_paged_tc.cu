@@ -63,8 +63,13 @@ constexpr int kItemRows = 2 * kTile;
 constexpr int kThreads = 512;
 constexpr int kMmaWarp = 8, kFetchWarp = 9, kConvWarp = 12;
 constexpr uint64_t kWaitNs = 2000000000ull;
-constexpr int kMaxSplit = 8;
+constexpr int kMaxSplit = kPagedMaxSplit;
 constexpr int kTmemCols = 512;
+
+// The largest power of two of V's scale that goes into the values of a slot: its product with the largest code (-128
+// among INT8's) is a finite FP16 value.
+template <int FMT>
+constexpr int kPowerMax = FMT == AF_KV_INT8 ? 8 : 7;
 
 template <int FMT, int HD>
 struct Shape {
@@ -79,10 +84,8 @@ struct Shape {
     static constexpr int kScales = kQuant ? kSlots / 2 + 1 : 1;
     static constexpr int kRing = kQBytes, kStaging = kRing + kSlots * kTileBytes;
     static constexpr size_t kSmem = kStaging + (size_t)kStages * kCodeBytes + 1024;   // + alignment to 1 KB
-    // The largest power of two of V's scale in a slot (times the largest code, -128 among INT8's, a finite FP16 value),
-    // and log2 of the growth of the maximum that forces a rescale: P times the rest of any finite scale stays finite in
-    // FP16 (2^7 * 511.75, 2^8 * 255.9).
-    static constexpr int kPowerMax = FMT == AF_KV_INT8 ? 8 : 7;
+    // log2 of the growth of the maximum that forces a rescale: P times the rest of any finite scale stays finite in FP16
+    // (2^7 * 511.75, 2^8 * 255.9).
     static constexpr float kGrow = FMT == AF_KV_FP8_E4M3 ? 7.f : 8.f;
     // the fetch ring: slots, or staging for codes
     static constexpr int kFetch = kQuant ? kStages : kSlots;
@@ -486,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const Paged p,
                 fetch(0);
                 for (int j = 0; j < n; ++j) {
                     // V's scale = power * rest, both exact; an infinity or NaN stays with the values, which are mended
-                    const KvScaleParts parts = kv_split_scale<FMT, Sh::kPowerMax>(__half2float(sv));
+                    const KvScaleParts parts = kv_split_scale<FMT, kPowerMax<FMT>>(__half2float(sv));
                     const bool odd = (__half_as_ushort(sv) & 0x7c00u) == 0x7c00u;
                     const uint32_t power = __half_as_ushort(odd ? sv : parts.power);
                     s_scale[j % Sh::kScales][0][mine] = sk;
@@ -962,23 +965,8 @@ cudaError_t paged_chunk_launch(int format, int head_dim, const Paged& p, const v
     const long long items = rows / kItemRows + seqs;
     const long long clusters = items * p.NKV;
     if (items == 0) return cudaSuccess;
-    // Split an item's positions over S CTAs where that shortens the whole: waves of CTAs x (tiles of each + what a CTA
-    // costs beside its tiles, about 3 tiles' time alone and 6 in a cluster that merges).  Clusters leave SMs out: of 148,
-    // cudaOccupancyMaxActiveClusters gives 148, 148, 132 and 120 to clusters of 1, 2, 4 and 8 such CTAs.
-    // (128 new tokens x 4 over 8192, 16 items: S = 8, 16 clusters for 15 places, 64 us; S = 4 47 us.)
     const long long full_items = std::max((rows + kItemRows - 1) / kItemRows, seqs) * p.NKV;
-    const int sms = std::max(8, device_sm_count()), tiles = std::max(1, (max_kv + kTile - 1) / kTile);
-    const int place[4] = {sms, sms / 2 * 2, sms * 33 / 148 * 4, sms * 15 / 148 * 8};
-    int S = 1;
-    double best = 1e300;
-    for (int i = 0; 1 << i <= kMaxSplit && (i == 0 || tiles >= 4 << i); ++i) {   // four tiles per CTA at least
-        const long long ctas = full_items << i, waves = (ctas + place[i] - 1) / place[i];
-        const double cost = (double)waves * ((double)tiles / (1 << i) + (i == 0 ? 3. : 6.));
-        if (cost < best) {
-            best = cost;
-            S = 1 << i;
-        }
-    }
+    const int S = paged_chunk_split(full_items, std::max(1, (max_kv + kTile - 1) / kTile), device_sm_count());
     if (clusters * S > 0x7fffffffll) return cudaErrorInvalidConfiguration;
     auto go = [&](auto fmt) {
         return head_dim == 128 ? launch<decltype(fmt)::value, 128>(p, a, (unsigned)clusters, S, fault, st)
