@@ -411,8 +411,7 @@ struct AttnPlan {
 };
 AttnPlan attn_plan(const Paged& p, int n_heads, int max_rows, int max_kv) {
     AttnPlan x;
-    const long long cap = (long long)p.max_pages << p.page_shift;
-    x.kv = (int)std::min<long long>({max_kv > 0 ? (long long)max_kv : cap, cap, INT_MAX});
+    x.kv = paged_kv_bound(max_kv, p.max_pages, p.page_shift);
     const int q = max_rows > 0 ? std::min(max_rows, p.n_tokens) : p.n_tokens;
     const long long rows = (long long)q * (n_heads / p.NKV);
     const bool even = (long long)q * p.n_seqs <= p.n_tokens;   // every sequence as long as the bound: none is short

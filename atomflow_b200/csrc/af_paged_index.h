@@ -18,11 +18,12 @@ struct PagedSeq {
     int row0, q, kv;
     bool bad;
 };
+constexpr int kPagedMaxKv = 1 << 30;   // of a sequence, so that a position plus a tile fits in an int
 // From the sequence's two row offsets and its length.  Rows outside [0, n_tokens),
-// decreasing offsets, a negative length or one beyond max_pages pages or 2^30
-// (so that a position plus a tile fits in an int): a bad sequence, without rows.
+// decreasing offsets, a negative length or one beyond max_pages pages or
+// kPagedMaxKv: a bad sequence, without rows.
 AF_HD PagedSeq paged_seq_of(int s, int e, int kv, int n_tokens, int max_pages, int page_shift) {
-    if (s < 0 || e < s || e > n_tokens || kv < 0 || kv > (1 << 30) || (int64_t)kv > ((int64_t)max_pages << page_shift))
+    if (s < 0 || e < s || e > n_tokens || kv < 0 || kv > kPagedMaxKv || (int64_t)kv > ((int64_t)max_pages << page_shift))
         return {0, 0, 0, true};
     return {s, e - s, kv, false};
 }
@@ -45,6 +46,13 @@ AF_HD int64_t paged_scale_at(int page, int64_t scale_stride, int slot, int nkv, 
     return (int64_t)page * scale_stride + (int64_t)slot * nkv + head;
 }
 
+
+// What a sequence's cached positions are at most: the caller's bound (0: none), the table, the largest length.
+inline int paged_kv_bound(int max_kv, int max_pages, int page_shift) {
+    int64_t n = (int64_t)max_pages << page_shift;
+    if (max_kv > 0 && max_kv < n) n = max_kv;
+    return n < kPagedMaxKv ? (int)n : kPagedMaxKv;
+}
 
 // Over how many CTAs (a power of two) the chunk kernel splits the positions of its work items, of at most `tiles` tiles
 // each, on a GPU of `sms` SMs (0 or less: not known): as many as shorten the whole, waves of CTAs x (tiles of each + what a

@@ -41,3 +41,22 @@ def test_the_split_of_148_sms(split):
     assert split(4, 64, 148) == 8 and split(1, 1000, 148) == 8
     assert split(148, 64, 148) == 1 and split(1000, 64, 148) == 1
     assert split(1, 7, 148) == 1 and split(1, 8, 148) == 2
+
+
+def test_the_bound_on_the_positions_leaves_room_for_a_tile(tmp_path):
+    """The caller's bound and the table's width may be as large as an int: the bound that the kernels' plans round up to
+    whole tiles is not."""
+    (tmp_path / "t.cpp").write_text('''
+#include "af_paged_index.h"
+extern "C" int bound(int max_kv, int pages, int shift) { return af::paged_kv_bound(max_kv, pages, shift); }''')
+    subprocess.run(["g++", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover", "-shared", "-fPIC", "-std=c++17", "-I",
+                    str(ROOT / "atomflow_b200" / "csrc"), "-o", str(tmp_path / "t.so"), str(tmp_path / "t.cpp"), "-lubsan"],
+                   check=True)
+    bound = ctypes.CDLL(str(tmp_path / "t.so")).bound
+    top, room = 2 ** 31 - 1, 2 ** 30
+    for max_kv in (0, 1, 100, 4096, room - 1, room, room + 1, top - 127, top):
+        for pages in (0, 1, 7, 2 ** 20, 2 ** 27, top):
+            for shift in (3, 4, 8):
+                want = min(max_kv or 2 ** 60, pages << shift, room)
+                assert bound(max_kv, pages, shift) == want
+                assert (want + 127) // 128 <= 2 ** 23
