@@ -10,6 +10,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -35,9 +36,11 @@ struct PythonError : std::exception {};   // already set
 
 [[noreturn]] void bad(const char* what) { throw ValueError(what); }
 
-// These operators serve; a gradient asked for would be lost without a word.
+// These operators serve; a gradient asked for, backward or forward (a dual tensor's tangent), would be lost without a word.
 void no_gradient(const at::Tensor& t) {
     if (t.requires_grad() && c10::GradMode::is_enabled()) bad("the paged operators have no gradient: detach the input, or call under torch.no_grad()");
+    if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
+        bad("the paged operators have no gradient: unpack the dual tensor, or call under torch.inference_mode()");
 }
 
 const at::Tensor& tensor(PyObject* o, const char* name) {
