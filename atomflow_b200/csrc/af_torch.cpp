@@ -19,6 +19,7 @@
 #include <climits>
 #include <cmath>
 #include <exception>
+#include <initializer_list>
 #include <stdexcept>
 #include <string>
 
@@ -37,6 +38,7 @@ struct PythonError : std::exception {};   // already set
 [[noreturn]] void bad(const char* what) { throw ValueError(what); }
 
 // These operators serve; a gradient asked for, backward or forward (a dual tensor's tangent), would be lost without a word.
+// Outputs given by the caller too: what is written into them is not recorded.
 void no_gradient(const at::Tensor& t) {
     if (t.requires_grad() && c10::GradMode::is_enabled()) bad("the paged operators have no gradient: detach the input, or call under torch.no_grad()");
     if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
@@ -60,6 +62,10 @@ int to_int(int64_t v, const char* what) {
     if (v < INT_MIN || v > INT_MAX) bad(what);
     return (int)v;
 }
+void no_gradient(std::initializer_list<const at::Tensor*> ts) {
+    for (const at::Tensor* t : ts)
+        if (t != nullptr) no_gradient(*t);
+}
 void* pointer(const at::Tensor& t) { return t.numel() == 0 ? nullptr : t.data_ptr(); }
 
 // The C structures of a cache and a batch, checked (shapes, types, strides, one device), and the device's index.
@@ -71,8 +77,7 @@ struct Paged {
 Paged paged(int64_t n_tokens, const at::Tensor& k, const at::Tensor& v, const at::Tensor& table, const at::Tensor& len,
             const at::Tensor& cu, const at::Tensor* ks, const at::Tensor* vs) {
     const char* one_device = "every tensor must be on one CUDA device";
-    for (const at::Tensor* t : {&k, &v, ks, vs})
-        if (t != nullptr) no_gradient(*t);
+    no_gradient({&k, &v, ks, vs});
     Paged p{};
     const at::ScalarType type = k.scalar_type();
     if (type == at::kHalf) p.kv.format = AF_KV_F16;
@@ -173,7 +178,7 @@ PyObject* paged_kv_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Tensor& qkv = tensor(a[0], "qkv");
         const at::Tensor *cos = optional(a[7], "cos"), *sin = optional(a[8], "sin"), *q_out = optional(a[11], "q_out");
         if (qkv.dim() != 2) bad("qkv must be [T, (n_heads + 2 n_kv_heads) * head_dim]");
-        no_gradient(qkv);
+        no_gradient({&qkv, cos, sin, q_out});
         const int64_t T = qkv.size(0), nh = integer(a[6]);
         Paged p = paged(T, tensor(a[1], "k_pages"), tensor(a[2], "v_pages"), tensor(a[3], "block_table"),
                         tensor(a[4], "kv_len"), tensor(a[5], "cu_rows"), optional(a[9], "k_scale"), optional(a[10], "v_scale"));
@@ -211,14 +216,16 @@ PyObject* paged_kv_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* paged_kv_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 10, [&]() -> PyObject* {
         const at::Tensor& pages = tensor(a[0], "k_pages");
+        const at::Tensor *k_out = optional(a[8], "k_out"), *v_out = optional(a[9], "v_out");
+        no_gradient({k_out, v_out});
         const int64_t T = integer(a[5]);
         if (T < 0) bad("n_rows must not be negative");
         Paged p = paged(T, pages, tensor(a[1], "v_pages"), tensor(a[2], "block_table"), tensor(a[3], "kv_len"),
                         tensor(a[4], "cu_rows"), optional(a[6], "k_scale"), optional(a[7], "v_scale"));
         const c10::cuda::CUDAGuard guard((c10::DeviceIndex)p.dev);
         const int64_t shape[3] = {T, p.kv.n_kv_heads, p.kv.head_dim};
-        const at::Tensor k = output(optional(a[8], "k_out"), "k_out", p.dev, shape, pages);
-        const at::Tensor v = output(optional(a[9], "v_out"), "v_out", p.dev, shape, pages);
+        const at::Tensor k = output(k_out, "k_out", p.dev, shape, pages);
+        const at::Tensor v = output(v_out, "v_out", p.dev, shape, pages);
         const af_status st = af_paged_kv_read(&p.kv, &p.batch, pointer(k), pointer(v),
                                               c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)p.dev).stream());
         if (st != AF_OK) return PyLong_FromLong(st);
@@ -235,7 +242,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 12, [&]() -> PyObject* {
         const at::Tensor& q = tensor(a[0], "q");
         if (q.dim() != 3) bad("q must be [T, n_heads, head_dim]");
-        no_gradient(q);
+        const at::Tensor* given = optional(a[11], "out");
+        no_gradient({&q, given});
         const int64_t T = q.size(0), nh = q.size(1);
         Paged p = paged(T, tensor(a[1], "k_pages"), tensor(a[2], "v_pages"), tensor(a[3], "block_table"),
                         tensor(a[4], "kv_len"), tensor(a[5], "cu_rows"), optional(a[7], "k_scale"), optional(a[8], "v_scale"));
@@ -254,7 +262,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         };
         const int max_q = bound(a[9], "max_q must not be negative"), max_kv = bound(a[10], "max_kv must not be negative");
         const c10::cuda::CUDAGuard guard((c10::DeviceIndex)p.dev);
-        const at::Tensor out = output(optional(a[11], "out"), "out", p.dev, {T, nh, hd}, q);
+        const at::Tensor out = output(given, "out", p.dev, {T, nh, hd}, q);
         const int heads = to_int(nh, "a dimension does not fit in 32 bits");
         // scratch of this call alone, from the stream's allocator: calls on several streams, or in several graphs,
         // share none

@@ -42,3 +42,22 @@ def test_tangents_are_refused():
         for call in calls(f16, {}, q, qkv):   # none among the arguments: the next check's refusal
             with pytest.raises(ValueError, match="CUDA device"):
                 call()
+
+
+def test_outputs_and_tables_that_require_a_gradient_are_refused():
+    from atomflow_b200 import ops
+    t, _, q = _t()
+    qkv, like = torch.zeros(1, 1024, dtype=torch.float16), torch.zeros(1, 2, 128, dtype=torch.float16)
+    tab = torch.zeros(8, 64)
+    grad = lambda x: x.clone().requires_grad_()
+    bad = [lambda: ops.paged_attention(q, **t, out=grad(q)),
+           lambda: ops.paged_kv_read(**t, n_rows=1, k_out=grad(like)),
+           lambda: ops.paged_kv_read(**t, n_rows=1, v_out=grad(like)),
+           lambda: ops.paged_kv_write(qkv, **t, n_heads=4, cos=grad(tab), sin=tab),
+           lambda: ops.paged_kv_write(qkv, **t, n_heads=4, cos=tab, sin=grad(tab)),
+           lambda: ops.paged_kv_write(qkv, **t, n_heads=4, cos=tab, sin=tab, q_out=grad(q))]
+    for call in bad:
+        with pytest.raises(ValueError, match="no gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="CUDA device"):   # there it is the caller's wish
+            call()
