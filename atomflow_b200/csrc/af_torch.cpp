@@ -66,6 +66,12 @@ void no_gradient(std::initializer_list<const at::Tensor*> ts) {
     for (const at::Tensor* t : ts)
         if (t != nullptr) no_gradient(*t);
 }
+// Tells autograd that tensors were written in place, so that what saved one for its backward pass notices.  (Tensors made
+// under inference mode have no version.)
+void written(std::initializer_list<const at::Tensor*> ts) {
+    for (const at::Tensor* t : ts)
+        if (t != nullptr && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
 void* pointer(const at::Tensor& t) { return t.numel() == 0 ? nullptr : t.data_ptr(); }
 
 // The C structures of a cache and a batch, checked (shapes, types, strides, one device), and the device's index.
@@ -180,8 +186,9 @@ PyObject* paged_kv_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (qkv.dim() != 2) bad("qkv must be [T, (n_heads + 2 n_kv_heads) * head_dim]");
         no_gradient({&qkv, cos, sin, q_out});
         const int64_t T = qkv.size(0), nh = integer(a[6]);
-        Paged p = paged(T, tensor(a[1], "k_pages"), tensor(a[2], "v_pages"), tensor(a[3], "block_table"),
-                        tensor(a[4], "kv_len"), tensor(a[5], "cu_rows"), optional(a[9], "k_scale"), optional(a[10], "v_scale"));
+        const at::Tensor &k = tensor(a[1], "k_pages"), &v = tensor(a[2], "v_pages");
+        const at::Tensor *ks = optional(a[9], "k_scale"), *vs = optional(a[10], "v_scale");
+        Paged p = paged(T, k, v, tensor(a[3], "block_table"), tensor(a[4], "kv_len"), tensor(a[5], "cu_rows"), ks, vs);
         const int64_t hd = p.kv.head_dim;
         if (nh < 0 || nh > INT_MAX) bad("n_heads must be a count of heads");
         const int64_t stride = rows(qkv, "qkv", p.dev, {T, (nh + 2 * p.kv.n_kv_heads) * hd});
@@ -207,6 +214,7 @@ PyObject* paged_kv_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                                to_int(max_seq, "the tables are too long"), q.defined() ? pointer(q) : nullptr,
                                                c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)p.dev).stream());
         if (st != AF_OK) return PyLong_FromLong(st);
+        written({&k, &v, ks, vs, q_out});
         if (!q.defined()) Py_RETURN_NONE;
         return THPVariable_Wrap(q);
     });
@@ -229,6 +237,7 @@ PyObject* paged_kv_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const af_status st = af_paged_kv_read(&p.kv, &p.batch, pointer(k), pointer(v),
                                               c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)p.dev).stream());
         if (st != AF_OK) return PyLong_FromLong(st);
+        written({k_out, v_out});
         PyObject *pk = THPVariable_Wrap(k), *pv = THPVariable_Wrap(v);
         PyObject* r = pk != nullptr && pv != nullptr ? PyTuple_Pack(2, pk, pv) : nullptr;
         Py_XDECREF(pk);
@@ -273,6 +282,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                                 pointer(out), need != 0 ? ws.data_ptr() : nullptr, need,
                                                 c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)p.dev).stream());
         if (st != AF_OK) return PyLong_FromLong(st);
+        written({given});
         return THPVariable_Wrap(out);
     });
 }
