@@ -6,9 +6,11 @@ nvcc cross-compiles without a GPU, so this runs on any machine with CUDA 12.8+.
 The shared CUDA runtime is linked so the library shares the process's current
 device and streams with any other CUDA user in the process (e.g. PyTorch).
 """
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -30,8 +32,14 @@ def headers():
             sorted((ROOT / "include").glob("*.h")))
 
 
+def torch_root():
+    """Where torch is installed; None: nowhere, and the torch module is not built."""
+    spec = importlib.util.find_spec("torch")
+    return None if spec is None else Path(spec.origin).parent
+
+
 def up_to_date() -> bool:
-    if not LIB.exists() or not CLI.exists() or not EXT.exists():
+    if not LIB.exists() or not CLI.exists() or (not EXT.exists() and torch_root() is not None):
         return False
     t = LIB.stat().st_mtime
     return all(p.stat().st_mtime <= t for p in sources() + headers())
@@ -76,13 +84,10 @@ def build(force: bool = False, verbose: bool = False) -> Path:
 
 def build_ext(verbose: bool = False) -> None:
     """The torch module over the C ABI; skipped where torch is not installed (the library itself does not need it)."""
-    import importlib.util
-    import sysconfig
-    spec = importlib.util.find_spec("torch")
-    if spec is None:
+    root = torch_root()
+    if root is None:
         return
     import torch
-    root = Path(spec.origin).parent
     cuda = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
     tmp = EXT.with_suffix(".so.tmp")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
