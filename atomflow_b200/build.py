@@ -33,9 +33,10 @@ def headers():
 
 
 def torch_root():
-    """Where torch is installed; None: nowhere, and the torch module is not built."""
+    """Where a torch built for CUDA is installed; None: nowhere, and the torch module is not built."""
     spec = importlib.util.find_spec("torch")
-    return None if spec is None else Path(spec.origin).parent
+    root = Path(spec.origin).parent if spec is not None and spec.origin else None
+    return root if root is not None and (root / "lib" / "libc10_cuda.so").exists() else None
 
 
 def up_to_date() -> bool:
@@ -83,9 +84,10 @@ def build(force: bool = False, verbose: bool = False) -> Path:
 
 
 def build_ext(verbose: bool = False) -> None:
-    """The torch module over the C ABI; skipped where torch is not installed (the library itself does not need it)."""
+    """The torch module over the C ABI; skipped where no torch built for CUDA is (the library itself does not need it)."""
     root = torch_root()
     if root is None:
+        print("no torch built for CUDA: _torch_ops.so is not built", file=sys.stderr)
         return
     import torch
     cuda = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))

@@ -81,3 +81,24 @@ def test_torch_installed_later(tree, monkeypatch):
         without_torch(m)
         assert tree.build() == LIBRARY
     assert tree.build()[-1] == "_torch_ops.so" and tree.build() == []
+
+
+def torch_at(monkeypatch, root, cuda):
+    """A torch under `root`, built for CUDA or not."""
+    (root / "lib").mkdir(parents=True, exist_ok=True)
+    for name, there in (("libc10.so", True), ("libc10_cuda.so", cuda)):
+        if there:
+            (root / "lib" / name).write_text("")
+    (root / "__init__.py").write_text("")
+    spec = importlib.machinery.ModuleSpec("torch", None, origin=str(root / "__init__.py"))
+    monkeypatch.setattr(importlib.util, "find_spec", lambda name, *a: spec)
+
+
+def test_a_torch_without_cuda_is_no_torch(tree, monkeypatch):
+    torch_at(monkeypatch, tree.tmp / "cpu_torch", cuda=False)
+    tree.fail = ("_torch_ops.so",)                   # there is no -lc10_cuda
+    assert tree.build() == LIBRARY
+    assert tree.build() == []
+    torch_at(monkeypatch, tree.tmp / "cuda_torch", cuda=True)
+    tree.fail = ()
+    assert tree.build()[-1] == "_torch_ops.so"
