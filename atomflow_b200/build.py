@@ -6,6 +6,7 @@ nvcc cross-compiles without a GPU, so this runs on any machine with CUDA 12.8+.
 The shared CUDA runtime is linked so the library shares the process's current
 device and streams with any other CUDA user in the process (e.g. PyTorch).
 """
+import importlib.metadata
 import importlib.util
 import os
 import subprocess
@@ -27,9 +28,17 @@ def sources():
     return sorted(CSRC.glob("*.cu"))
 
 
+def public_headers():
+    return sorted((ROOT / "include").glob("*.h"))
+
+
+def ext_source():
+    return CSRC / "af_torch.cpp"
+
+
 def headers():
-    return (sorted(CSRC.glob("*.h")) + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.cpp")) +
-            sorted((ROOT / "include").glob("*.h")))
+    programs = [p for p in sorted(CSRC.glob("*.cpp")) if p != ext_source()]
+    return sorted(CSRC.glob("*.h")) + sorted(CSRC.glob("*.cuh")) + programs + public_headers()
 
 
 def torch_root():
@@ -39,11 +48,40 @@ def torch_root():
     return root if root is not None and (root / "lib" / "libc10_cuda.so").exists() else None
 
 
+def torch_version() -> str:
+    try:
+        return importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:   # a torch on the path that no package manager put there
+        return str(torch_root())
+
+
+def ext_key() -> str:
+    """What the torch module fits besides its sources: this torch, this Python."""
+    return f"torch {torch_version()}, {sysconfig.get_config_var('SOABI')}"
+
+
+def ext_stamp() -> Path:
+    """Holds the ext_key of the module that was built last."""
+    return PKG / "_build" / "torch_ops.txt"
+
+
+def newer(target: Path, inputs) -> bool:
+    return target.exists() and all(p.stat().st_mtime <= target.stat().st_mtime for p in inputs)
+
+
+def lib_up_to_date() -> bool:
+    return all(newer(t, sources() + headers()) for t in (LIB, CLI))
+
+
+def ext_up_to_date() -> bool:
+    if torch_root() is None:
+        return True
+    return (newer(EXT, [ext_source()] + public_headers()) and ext_stamp().exists() and
+            ext_stamp().read_text() == ext_key())
+
+
 def up_to_date() -> bool:
-    if not LIB.exists() or not CLI.exists() or (not EXT.exists() and torch_root() is not None):
-        return False
-    t = LIB.stat().st_mtime
-    return all(p.stat().st_mtime <= t for p in sources() + headers())
+    return lib_up_to_date() and ext_up_to_date()
 
 
 # Translation units whose element-wise arithmetic must round exactly like the
@@ -53,8 +91,15 @@ FAST_MATH = {"af_decode.cu"}
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    if not force and up_to_date():
-        return LIB
+    if force or not lib_up_to_date():
+        build_lib(verbose)
+    if force or not ext_up_to_date():
+        build_ext(verbose)
+    return LIB
+
+
+def build_lib(verbose: bool = False) -> None:
+    """The library and the C++ program on it."""
     nvcc = os.environ.get("NVCC", "nvcc")
     tmp = LIB.with_suffix(".so.tmp")
     objdir = PKG / "_build"
@@ -79,8 +124,6 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     if verbose:
         print(" ".join(cmd))
     subprocess.run(cmd, check=True, cwd=str(PKG))
-    build_ext(verbose)
-    return LIB
 
 
 def build_ext(verbose: bool = False) -> None:
@@ -103,6 +146,8 @@ def build_ext(verbose: bool = False) -> None:
         print(" ".join(cmd))
     subprocess.run(cmd, check=True, cwd=str(PKG))
     os.replace(tmp, EXT)
+    ext_stamp().parent.mkdir(exist_ok=True)
+    ext_stamp().write_text(ext_key())
 
 
 if __name__ == "__main__":

@@ -102,3 +102,39 @@ def test_a_torch_without_cuda_is_no_torch(tree, monkeypatch):
     torch_at(monkeypatch, tree.tmp / "cuda_torch", cuda=True)
     tree.fail = ()
     assert tree.build()[-1] == "_torch_ops.so"
+
+
+def test_the_module_is_rebuilt_for_another_torch_or_python(tree, monkeypatch):
+    pytest.importorskip("torch")
+    tree.build()
+    monkeypatch.setattr(B, "torch_version", lambda: "99.0", raising=False)
+    assert tree.build() == ["_torch_ops.so"] and tree.build() == []
+
+
+def test_a_module_that_failed_to_compile_is_not_fresh(tree):
+    """The library is replaced before the module is compiled: the old module beside the new library is stale."""
+    pytest.importorskip("torch")
+    tree.build()
+    tree.touch(B.ROOT / "include" / "atomflow_b200.h")
+    tree.fail = ("_torch_ops.so",)
+    with pytest.raises(subprocess.CalledProcessError):
+        tree.build()
+    tree.fail = ()
+    assert tree.build() == ["_torch_ops.so"] and tree.build() == []
+
+
+def test_a_program_that_failed_to_link_is_not_fresh(tree):
+    tree.build()
+    tree.touch(B.CSRC / "a.h")
+    tree.fail = ("af_generate",)
+    with pytest.raises(subprocess.CalledProcessError):
+        tree.build()
+    tree.fail = ()
+    assert "af_generate" in tree.build() and tree.build() == []
+
+
+def test_only_the_module_depends_on_its_source(tree):
+    pytest.importorskip("torch")
+    tree.build()
+    tree.touch(B.CSRC / "af_torch.cpp")
+    assert tree.build() == ["_torch_ops.so"] and tree.build() == []
