@@ -2,8 +2,9 @@
 // drafted ones) over a paged KV cache: af_paged_attention's path for sequences
 // of at most 16 (token, query head) rows per kv head.
 //
-// Bound by reading the cache once (one token over 131,001 FP8 positions, 8 heads of 128:
-// 54 us, 5.1 TB/s; 64 ragged INT8 sequences of up to 8000: 126 us, 5.1 TB/s).  An item is one (sequence, kv head); its
+// The floor is reading the cache once (one token over 131,001 FP8 positions, 8 heads of 128:
+// 54.5 us in a graph, 58.5 to 59.5 among other calls, 5.0 and 4.6 TB/s; 64 ragged INT8 sequences of up to 8000: 127 us,
+// 5.1 TB/s, and 133 to 143).  An item is one (sequence, kv head); its
 // positions go in tiles of 16, each of a CTA's W warps taking every W-th tile of
 // the CTA's range in a cp.async ring of its own (no CTA-wide barrier in the loop).
 // The work is divided over CTAs in one of two ways:
@@ -30,6 +31,8 @@
 //     1152.  (Left in the operand and taken out of the accumulator as 1152 sum(q),
 //     the offset costs no instruction, but the accumulator then rounds at its
 //     size, up to 2^10 times the score's for a query that leans to one side.)
+//   * P is rounded to FP16, the second MMA's operand (relative error of the output
+//     2.7e-4 to 2.9e-4, where its own rounding alone makes 2.1e-4).
 //   * K's scale multiplies S in FP32.  V's is split: its power of two into the
 //     codes' FP16 operands, exactly, the rest, in [1, 2), into P before its one
 //     rounding.  A position's weight so keeps its 11 bits whatever the scales
@@ -37,10 +40,10 @@
 //     of the warp's, one vector of zeros, whose scale is 1, left the others'
 //     weights the bits of FP16's subnormals.)
 //   * Warps and CTAs merge in a fixed order: the same bits every time.
-//   * The loop is bound by issue slots as much as by DRAM: 8 warps per SM (two per
+//   * The loop is bound by the latency of a warp's steps: 8 warps per SM (two per
 //     scheduler) issued in 45% of the cycles and read the cache at 3.6 TB/s, so
 //     the rings are short and the registers few enough for 16 (12 with 16 rows
-//     of 128 dims).
+//     of 128 dims), which issue in 56 to 58% and keep DRAM 63% busy.
 #include <cooperative_groups.h>
 
 #include <algorithm>

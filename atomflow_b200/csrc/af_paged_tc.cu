@@ -14,8 +14,8 @@
 //     128-byte-swizzled layout that the MMA reads; a page outside the pool is a
 //     coordinate outside the tensor, which reads as zeros.  8-bit codes land in a
 //     staging ring, and warps 12-15 turn them into FP16 slots exactly: K's codes as
-//     they are, V's times their scale's power of two.  The rest of the scales is
-//     applied in FP32 by the softmax, K's to the columns of S, V's (in [1, 2)) to P
+//     they are, V's times their scale's power of two (kv_split_scale).  The rest of the scales is
+//     applied in FP32 by the softmax, K's to the columns of S, V's (in [1, 2) for the scales that the write stores) to P
 //     before its rounding: multiplied into the FP16 slots they cost a rounding
 //     of every element (relative error against 64 bits of a 4096-token FP8 prompt
 //     3.9e-4, 130 us; as it is 2.7e-4, 152 us; FP32 scales in shared memory 152 us).
@@ -33,16 +33,21 @@
 //     is in its softmax.
 //   * Warps 0-3 and 4-7 load Q and are the softmax of row tile 0 and 1, one row per
 //     thread: no shuffles.  O is rescaled only when the row's maximum has grown by more
-//     than a factor 2^8 since the last rescale (P then stays below 2^8, exact
+//     than a factor 2^8 (FP8 2^7) since the last rescale (P then stays below that, exact
 //     range in FP16; l and O are FP32), which ends after the first few tiles.
-//   * P is rounded to FP16 for the second product: its error, 2^-12 of each
-//     weight on average, is that of the FP16 output's own rounding.
+//   * P is rounded to FP16 for the second product, the type of V's tile: its error, at most 2^-11 of each
+//     weight, is that of the FP16 output's own rounding (relative error 2.7e-4 to 2.9e-4, without it 2.1e-4).
 //   * Few rows and a long cache: a work item's positions are split over the CTAs
 //     of a cluster, which merge through distributed shared memory in rank order
 //     -- no workspace, no second launch, the same bits every time.
 //   * Bound: FP16 by the MMAs, which share shared memory's bandwidth with TMA (4 x 1024
-//     new tokens over 16384, 32 heads over 8: 1113-1150 us, 925-957 TFLOP/s); 8 bits by the
-//     softmax's issue slots too (4096-token FP8 prompt, 24 heads: 153 us, 674 TFLOP/s).
+//     new tokens over 16384, 32 heads over 8: 1131 to 1148 us in a graph, 1167 to 1175 among other calls, 906 to 942
+//     TFLOP/s); 8 bits by the chain S, softmax of all columns, P V, next S in the same columns, which two row tiles do
+//     not cover once the scales lengthen the softmax (4096-token FP8 prompt, 24 heads: 153 us, 674 TFLOP/s; issue
+//     slots 46% used, tensor pipe 34%).
+//   * Registers: 128 at launch, 184 in the softmax warps.  -Xptxas -v counts 76 to 92 bytes of spills: values that the
+//     cluster's merge needs after the loop (without that part four of the six variants have none, the others 44 and
+//     52).  The rest of the 152-byte frame belongs to the calls of add_mended.
 //   * Every wait is bounded; one that runs out sets AF_FAULT_TC_WAIT and the
 //     kernel ends without waiting further.
 #include <cooperative_groups.h>

@@ -112,6 +112,10 @@ def argmax(logits, *, mode="true", out=None, workspace=None, stream=None):
 # ------------------------------------------------------------ paged KV cache
 # Checks, outputs and the call of the C ABI are in the module _torch_ops (csrc/af_torch.cpp): a decode step calls these
 # for every layer, and in Python they took longer than the kernels.
+#
+# stream: a torch.cuda.Stream of the pages' device, the current one unless given.  As with the other ops nothing is
+# recorded on it: the caller orders it behind the streams that made the inputs and keeps those alive until it is done; new
+# outputs are allocated on it.  No gradients: inputs, tables and given outputs that ask for one are refused.
 _native = None
 
 
@@ -138,7 +142,7 @@ def paged_kv_write(qkv, k_pages, v_pages, block_table, kv_len, cu_rows, *, n_hea
                    v_scale=None, q_out=None, stream=None):
     """Stores a batch's new tokens in their pages (quantised, in 8-bit pages); in place.
 
-    qkv fp16 [T, (n_heads + 2 * n_kv_heads) * head_dim], rows any distance apart.  With
+    qkv fp16 [T, (n_heads + 2 * n_kv_heads) * head_dim], rows any multiple of 8 elements apart.  With
     RoPE tables (fp32 [max_seq, head_dim / 2]) q and k are rotated at the tokens'
     positions; returns q [T, n_heads, head_dim]: rotated in q_out, or without tables
     qkv's own q.  The cache and the batch (int32 block_table [n_seqs, max_pages], kv_len
@@ -174,9 +178,10 @@ def paged_attention(q, k_pages, v_pages, block_table, kv_len, cu_rows, *, scale=
                     max_q=None, max_kv=None, out=None, stream=None):
     """Causal attention of a batch's new tokens over their cached positions, themselves included.
 
-    q fp16 [T, n_heads, head_dim], tokens any distance apart; returns out, alike and
+    q fp16 [T, n_heads, head_dim], tokens any multiple of 8 elements apart; returns out, alike and
     contiguous.  scale: 1 / sqrt(head_dim) unless given.  max_q, max_kv: the host's bounds on
-    any sequence's new tokens and cached positions, which choose the split of the work."""
+    any sequence's new tokens and cached positions, which choose the split of the work (a sequence
+    of more tokens than max_q may be left out, which af_device_faults tells)."""
     if stream is not None:
         with _on_stream(stream, k_pages.device):
             return paged_attention(q, k_pages, v_pages, block_table, kv_len, cu_rows, scale=scale, k_scale=k_scale,

@@ -360,7 +360,8 @@ af_status af_gemv_chain_fast(const af_chain_op* ops, int n_ops, void* workspace,
  *                       and rounded to FP16; q goes to q_out [n_tokens][NH][HD]
  *                       (not overlapping qkv), k and v to the pages.  A position
  *                       outside the tables sets AF_FAULT_POSITION and skips its
- *                       row.  Tables NULL: k and v are stored as they are, q is
+ *                       row; so does a page outside the pool: that row of q_out
+ *                       is left as it was.  Tables NULL: k and v are stored as they are, q is
  *                       left alone (q_out may be NULL).
  *   af_paged_kv_read    the rows' positions as FP16 k_out, v_out
  *                       [n_tokens][NKV][HD] (cu_rows = sums of kv_len: whole
@@ -370,7 +371,8 @@ af_status af_gemv_chain_fast(const af_chain_op* ops, int n_ops, void* workspace,
  *                       code * scale not rounded to FP16, whatever finite scale a
  *                       caller's own pool has), q FP16 [n_tokens] rows
  *                       [NH][HD] q_stride elements apart (a multiple of 8), out
- *                       FP16 [n_tokens][NH][HD], NH % NKV == 0.  max_rows and
+ *                       FP16 [n_tokens][NH][HD], NH % NKV == 0, scale positive and
+ *                       finite.  max_rows and
  *                       max_kv are the host's bounds on a sequence's rows and
  *                       positions (0: not known): they choose how the work is
  *                       split, never the result's meaning.  A sequence of more
